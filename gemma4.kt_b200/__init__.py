@@ -17,3 +17,4 @@ from .floattensor import (  # noqa: F401
 )
 from .moe import FfnMoeBlock, MoeLayer, topk  # noqa: F401
 from .model import DecoderBatch, DecoderModel, DecoderState, ModelConfig, TensorSource  # noqa: F401
+from .paged import KvCache, Rope, beam_select  # noqa: F401

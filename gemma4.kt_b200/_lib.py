@@ -24,6 +24,7 @@ ERRORS = {
 
 # Every symbol include/g4.h declares, with its ctypes signature.
 _vp, _i, _i64, _u64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float
+_sz = C.c_size_t
 SIGNATURES = {
     "g4_init": (_i, [_i, C.POINTER(_vp)]),
     "g4_destroy": (_i, [_vp]),
@@ -70,6 +71,26 @@ SIGNATURES = {
     "g4_batch_step": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp]),
     "g4_batch_stream": (_vp, [_vp]),
     "g4_batch_expert_parallel": (_i, [_vp]),
+    "g4_kv_create": (_i, [_vp, _vp, C.POINTER(_vp)]),
+    "g4_kv_free": (_i, [_vp]),
+    "g4_kv_k": (_vp, [_vp, _i]),
+    "g4_kv_v": (_vp, [_vp, _i]),
+    "g4_kv_table": (_vp, [_vp]),
+    "g4_kv_lens": (_vp, [_vp]),
+    "g4_kv_refs": (_vp, [_vp]),
+    "g4_kv_resize": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "g4_kv_fork": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "g4_kv_compact": (_i, [_vp, _vp]),
+    "g4_kv_copy_pages": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "g4_kv_check": (_i, [_vp, C.POINTER(_i), _vp]),
+    "g4_rope_create": (_i, [_vp, _vp, C.POINTER(_vp)]),
+    "g4_rope_free": (_i, [_vp]),
+    "g4_rope_apply": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _vp, _i, _vp]),
+    "g4_kv_append": (_i, [_vp, _i, _vp, _vp, _vp]),
+    "g4_kv_attend_workspace": (_sz, [_vp, _i]),
+    "g4_kv_attend": (_i, [_vp, _i, _vp, _vp, _sz, _vp]),
+    "g4_beam_select_workspace": (_sz, [_i, _i, _i]),
+    "g4_beam_select": (_i, [_vp, _vp, _i64, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 
@@ -112,6 +133,39 @@ class ModelConfigStruct(C.Structure):
                [(n, C.c_float) for n in ("eps", "rope_theta", "rope_theta_swa", "logit_softcap")] + \
                [(n, C.c_int) for n in ("n_expert", "n_expert_used", "expert_ff")] + \
                [("n_kv_heads", C.c_void_p), ("ff", C.c_void_p), ("is_swa", C.c_void_p)]
+
+
+class KvConfigStruct(C.Structure):
+    """g4_kv_config (include/g4.h)."""
+
+    _fields_ = [("n_layers", C.c_int), ("n_kv_heads", C.c_void_p), ("head_size", C.c_void_p)] + \
+               [(n, C.c_int) for n in ("type", "page_size", "n_pages", "n_seqs", "max_positions")]
+
+
+class RopeConfigStruct(C.Structure):
+    """g4_rope_config (include/g4.h)."""
+
+    _fields_ = [(n, C.c_int) for n in ("head_size", "rot_dim", "layout", "scaling")] + \
+               [("theta", C.c_double), ("factor", C.c_double), ("original_ctx", C.c_int), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("attn_factor", C.c_double), ("freq_factors", C.c_void_p)]
+
+
+class KvRowsStruct(C.Structure):
+    """g4_kv_rows (include/g4.h)."""
+
+    _fields_ = [("n_rows", C.c_int), ("n_heads", C.c_int)] + \
+               [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + \
+               [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + \
+               [(n, C.c_void_p) for n in ("seqs", "pos", "q_norm", "k_norm")] + \
+               [("norm_v", C.c_int), ("eps", C.c_float)]
+
+
+class KvQueriesStruct(C.Structure):
+    """g4_kv_queries (include/g4.h)."""
+
+    _fields_ = [("n_rows", C.c_int), ("n_heads", C.c_int), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_int64), ("out_stride", C.c_int64), ("seqs", C.c_void_p), ("pos", C.c_void_p),
+                ("scale", C.c_float), ("window", C.c_int), ("sinks", C.c_int)]
 
 
 _lib = None

@@ -3,6 +3,7 @@
 #include "g4.h"
 #include "g4_ctx.h"
 #include "g4_gemv.cuh"
+#include "g4_kv.h"
 
 #include <dlfcn.h>
 #include <nccl.h>
@@ -152,6 +153,9 @@ int g4_init(int device, g4_ctx** out) {
   // otherwise appear at its first use, after a host may have reserved the
   // remaining HBM.  A failure here is reported by that entry point later.
   noalloc_prepare_device(device);
+  // g4_beam_select has no handle to create: load its kernels now, so that its
+  // first call may be captured (a failure comes back at the launch).
+  if (beam_prepare()) cudaGetLastError();
   *out = c;
   return 0;
 }

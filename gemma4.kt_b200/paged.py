@@ -1,0 +1,318 @@
+"""Paged serving: a KV cache whose pages sequences share (g4_kv), rotary
+positions (g4_rope), attention over the cache and beam search's selection.
+
+The reference keeps one contiguous cache per LlamaState
+(model/LlamaState.kt:38-77) and samples one sequence (sampler/Sampler.kt);
+these are the operators a server or a beam search needs next to the decoder:
+
+    cache.fork(src, dst)               beams share their parent's pages
+    cache.resize(seqs, lens)           one more position each
+    cache.append(layer, q, k, v, ...)  norms, rotary positions, K/V rows
+    cache.attend(layer, q, out, ...)   softmax(q k) v over the pages
+    beam_select(ctx, logits, ...)      the next beams, parents for fork
+
+Tensors are torch CUDA tensors on the context's device; every call is
+asynchronous on `stream` (default: torch's current stream of that device) and
+may be captured into a CUDA graph.  What a call finds wrong in device data is
+skipped and reported by KvCache.check().
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from ._lib import KvConfigStruct, KvQueriesStruct, KvRowsStruct, RopeConfigStruct, check, lib
+from .floattensor import Context, GGMLType, UnsupportedOperation
+
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+
+
+def _stream(ctx: Context, stream):
+    if stream is not None:
+        return int(stream)
+    import torch
+
+    return torch.cuda.current_stream(ctx.device).cuda_stream
+
+
+def _workspace(ctx: Context, n: int, stream):
+    """n bytes from torch's allocator, in the pool of the stream that uses them."""
+    import torch
+
+    if stream is None:
+        return torch.empty(n, dtype=torch.uint8, device=f"cuda:{ctx.device}")
+    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=ctx.device)):
+        return torch.empty(n, dtype=torch.uint8, device=f"cuda:{ctx.device}")
+
+
+def _tensor(ctx: Context, t, name: str, dtype, rows: int | None = None, width: int | None = None):
+    """Check a tensor of `rows` entries, or (width given) of rows x width with
+    any row stride; returns (address, floats between rows)."""
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError(f"{name} must be a CUDA tensor on device {ctx.device}, got {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if width is None:
+        if (rows is not None and t.numel() != rows) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous with {rows} entries, got {tuple(t.shape)}")
+        return t.data_ptr(), 0
+    if t.dim() != 2 or t.shape[1] != width or t.shape[0] != rows or (width > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [{rows}, {width}] with consecutive columns, got {tuple(t.shape)}")
+    return t.data_ptr(), t.stride(0)
+
+
+class _Owner:
+    """Frees a handle when the last object that uses its memory is gone."""
+
+    def __init__(self, handle, release):
+        self.handle, self.release = handle, release
+
+    def free(self) -> None:
+        if self.handle:
+            self.release(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class _DeviceArray:
+    """Device memory of a cache for torch.as_tensor (the tensor keeps its owner alive)."""
+
+    def __init__(self, owner, ptr: int, shape, typestr: str):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(shape), "typestr": typestr, "version": 2}
+
+
+class Rope:
+    """A rotary plan (g4_rope).  layout "half" pairs element m with m + rot_dim/2,
+    "interleaved" 2m with 2m + 1; scaling "none", "linear" or "yarn" for
+    contexts `factor` times longer; freq_factors: the model's rope_freqs."""
+
+    def __init__(self, ctx: Context, head_size: int, rot_dim: int | None = None, theta: float = 10000.0,
+                 layout: str = "half", scaling: str = "none", factor: float = 1.0, original_ctx: int = 4096,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0, freq_factors=None):
+        if layout not in _LAYOUTS or scaling not in _SCALINGS:
+            raise ValueError(f"layout {layout!r} (half, interleaved), scaling {scaling!r} (none, linear, yarn)")
+        rot_dim = head_size if rot_dim is None else rot_dim
+        ff = None if freq_factors is None else np.ascontiguousarray(freq_factors, np.float32)
+        if ff is not None and ff.size != rot_dim // 2:
+            raise ValueError(f"freq_factors must hold {rot_dim // 2} values, got {ff.size}")
+        cfg = RopeConfigStruct(head_size, rot_dim, _LAYOUTS[layout], _SCALINGS[scaling], theta, factor, original_ctx,
+                               beta_fast, beta_slow, attn_factor, None if ff is None else ff.ctypes.data)
+        h = C.c_void_p()
+        rc = lib().g4_rope_create(ctx.handle, C.byref(cfg), C.byref(h))
+        if rc == -1:
+            raise ValueError(ctx.last_error())
+        check(rc, ctx.handle, "g4_rope_create")
+        self.ctx, self.head_size, self.handle = ctx, head_size, h
+        self._owner = _Owner(h, lib().g4_rope_free)
+
+    def free(self) -> None:
+        self.handle = None
+        self._owner.free()
+
+    def apply(self, x, out, pos, stream=None) -> None:
+        """out = x [rows, heads * head_size] (fp32) rotated at positions pos
+        [rows] (int32); out may be x; rows at negative positions stay."""
+        import torch
+
+        rows, width = x.shape if x.dim() == 2 else (0, 0)
+        if x.dim() != 2 or width % self.head_size or not width:
+            raise ValueError(f"x must be [rows, heads * {self.head_size}], got {tuple(x.shape)}")
+        xp, xs = _tensor(self.ctx, x, "x", torch.float32, rows, width)
+        op, os_ = _tensor(self.ctx, out, "out", torch.float32, rows, width)
+        pp, _ = _tensor(self.ctx, pos, "pos", torch.int32, rows)
+        check(lib().g4_rope_apply(self.handle, xp, xs, op, os_, width // self.head_size, pp, rows,
+                                  _stream(self.ctx, stream)), self.ctx.handle, "g4_rope_apply")
+
+
+class KvCache:
+    """A paged KV cache (g4_kv): n_pages pages of page_size positions in every
+    layer, shared by up to n_seqs sequences of at most max_positions."""
+
+    def __init__(self, ctx: Context, n_kv_heads, head_size, dtype=GGMLType.BF16, page_size: int = 32,
+                 n_pages: int = 1024, n_seqs: int = 64, max_positions: int = 4096):
+        heads, sizes = np.array(n_kv_heads, np.int32), np.array(head_size, np.int32)
+        if heads.ndim != 1 or heads.shape != sizes.shape or not heads.size:
+            raise ValueError("n_kv_heads and head_size must list the same layers")
+        cfg = KvConfigStruct(heads.size, heads.ctypes.data, sizes.ctypes.data, int(dtype), page_size, n_pages, n_seqs,
+                             max_positions)
+        h = C.c_void_p()
+        rc = lib().g4_kv_create(ctx.handle, C.byref(cfg), C.byref(h))
+        if rc == -2:
+            raise UnsupportedOperation(ctx.last_error())
+        if rc == -1:
+            raise ValueError(ctx.last_error())
+        check(rc, ctx.handle, "g4_kv_create")
+        self.ctx, self.handle = ctx, h
+        self._owner = _Owner(h, lib().g4_kv_free)
+        self.n_kv_heads, self.head_size = [int(x) for x in heads], [int(x) for x in sizes]
+        self.dtype, self.page_size, self.n_pages, self.n_seqs = GGMLType(int(dtype)), page_size, n_pages, n_seqs
+        self.max_positions, self.max_pages = max_positions, -(-max_positions // page_size)
+        self._work = [lib().g4_kv_attend_workspace(h, l) for l in range(heads.size)]
+        self._views = {}
+
+    def free(self) -> None:
+        """Release the pages (no view of them is used afterwards)."""
+        self._views.clear()
+        self.handle = None
+        self._owner.free()
+
+    # ---- the device state as tensors
+    def _view(self, key, ptr, shape, typestr: str):
+        t = self._views.get(key)
+        if t is None:
+            import torch
+
+            at = ptr()
+            if not at:
+                raise ValueError(f"no {key[0]} {key[1:]} in this cache")
+            t = torch.as_tensor(_DeviceArray(self._owner, at, shape, typestr), device=f"cuda:{self.ctx.device}")
+            if typestr == "<i2":
+                t = t.view(torch.bfloat16)
+            self._views[key] = t
+        return t
+
+    def _pool(self, name: str, layer: int):
+        kind = {GGMLType.F32: "<f4", GGMLType.F16: "<f2", GGMLType.BF16: "<i2"}[self.dtype]
+        if not 0 <= layer < len(self.head_size):
+            raise ValueError(f"layer {layer} of {len(self.head_size)}")
+        return self._view((name, layer), lambda: getattr(lib(), "g4_kv_" + name)(self.handle, layer),
+                          (self.n_pages, self.n_kv_heads[layer], self.page_size, self.head_size[layer]), kind)
+
+    def k(self, layer: int):
+        """K rows of a layer: [n_pages, n_kv_heads, page_size, head_size]."""
+        return self._pool("k", layer)
+
+    def v(self, layer: int):
+        """V rows of a layer: [n_pages, n_kv_heads, page_size, head_size]."""
+        return self._pool("v", layer)
+
+    @property
+    def table(self):
+        """Page of each position range of each sequence [n_seqs, max_pages], -1: none."""
+        return self._view(("table",), lambda: lib().g4_kv_table(self.handle), (self.n_seqs, self.max_pages), "<i4")
+
+    @property
+    def lens(self):
+        """Positions each sequence has pages for [n_seqs]."""
+        return self._view(("lens",), lambda: lib().g4_kv_lens(self.handle), (self.n_seqs,), "<i4")
+
+    @property
+    def refs(self):
+        """Sequences that hold each page [n_pages]."""
+        return self._view(("refs",), lambda: lib().g4_kv_refs(self.handle), (self.n_pages,), "<i4")
+
+    # ---- pages
+    def _pairs(self, fn, a, b, names, stream):
+        import torch
+
+        n = a.numel()
+        ap, _ = _tensor(self.ctx, a, names[0], torch.int32, n)
+        bp, _ = _tensor(self.ctx, b, names[1], torch.int32, n)
+        check(getattr(lib(), fn)(self.handle, ap, bp, n, _stream(self.ctx, stream)), self.ctx.handle, fn)
+
+    def resize(self, seqs, lens, stream=None) -> None:
+        """Pages for lens[i] positions of sequence seqs[i] (int32 tensors; 0 frees
+        it); a shared, partly filled last page is copied when a sequence grows
+        into it.  Without enough free pages nothing changes (check())."""
+        self._pairs("g4_kv_resize", seqs, lens, ("seqs", "lens"), stream)
+
+    def fork(self, src, dst, stream=None) -> None:
+        """Sequence dst[i] shares the pages of src[i] as they were before the call
+        (its own are given back); negative entries are padding."""
+        self._pairs("g4_kv_fork", src, dst, ("src", "dst"), stream)
+
+    def copy_pages(self, src, dst, stream=None) -> None:
+        """Whole pages src[i] -> dst[i] in every layer."""
+        self._pairs("g4_kv_copy_pages", src, dst, ("src", "dst"), stream)
+
+    def compact(self, stream=None) -> None:
+        """Live pages to the front of the pool; the table follows."""
+        check(lib().g4_kv_compact(self.handle, _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_compact")
+
+    def check(self, stream=None) -> int:
+        """Wait for the stream; raise what the cache's calls recorded, else the
+        number of free pages."""
+        n = C.c_int()
+        check(lib().g4_kv_check(self.handle, C.byref(n), _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_check")
+        return n.value
+
+    # ---- rows
+    def append(self, layer: int, q, k, v, q_out, seqs, pos, rope: Rope | None = None, q_norm=None, k_norm=None,
+               v_norm: bool = False, eps: float = 1e-6, stream=None) -> None:
+        """Row i is position pos[i] of sequence seqs[i]: its K and V rows, normed
+        and rotated, go into their page, its normed and rotated queries to q_out
+        (which may be q; q and q_out None: K and V alone).  fp32 rows
+        [rows, heads * head_size] with any row stride."""
+        import torch
+
+        f32, n = torch.float32, pos.numel()
+        if not 0 <= layer < len(self.head_size):
+            raise ValueError(f"layer {layer} of {len(self.head_size)}")
+        hs, width = self.head_size[layer], self.n_kv_heads[layer] * self.head_size[layer]
+        kp, ks = _tensor(self.ctx, k, "k", f32, n, width)
+        vp, vs = _tensor(self.ctx, v, "v", f32, n, width)
+        heads = qp = qs = op = os_ = 0
+        if q is not None:
+            if q.dim() != 2 or q.shape[1] % hs or not q.shape[1]:
+                raise ValueError(f"q must be [rows, heads * {hs}], got {tuple(q.shape)}")
+            heads = q.shape[1] // hs
+            qp, qs = _tensor(self.ctx, q, "q", f32, n, q.shape[1])
+            op, os_ = _tensor(self.ctx, q_out, "q_out", f32, n, q.shape[1])
+        norms = [_tensor(self.ctx, w, "norm weight", f32, hs)[0] if w is not None else None for w in (q_norm, k_norm)]
+        rows = KvRowsStruct(n, heads, qp or None, kp, vp, op or None, qs, ks, vs, os_,
+                            _tensor(self.ctx, seqs, "seqs", torch.int32, n)[0],
+                            _tensor(self.ctx, pos, "pos", torch.int32, n)[0], *norms, int(bool(v_norm)), eps)
+        check(lib().g4_kv_append(self.handle, layer, C.byref(rows), rope.handle if rope is not None else None,
+                                 _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_append")
+
+    def attend(self, layer: int, q, out, seqs, pos, scale: float = 1.0, window: int = 0, sinks: int = 0,
+               stream=None) -> None:
+        """out[i] = softmax(scale * q[i] . K) V over the positions t <= pos[i] of
+        sequence seqs[i]; with a window those above pos[i] - window and the first
+        `sinks`.  fp32 rows [rows, heads * head_size] with any row stride; rows
+        of negative sequences stay, rows at negative positions get zeros."""
+        import torch
+
+        f32, n = torch.float32, pos.numel()
+        if not 0 <= layer < len(self.head_size):
+            raise ValueError(f"layer {layer} of {len(self.head_size)}")
+        hs = self.head_size[layer]
+        if q.dim() != 2 or q.shape[1] % hs or not q.shape[1]:
+            raise ValueError(f"q must be [rows, heads * {hs}], got {tuple(q.shape)}")
+        qp, qs = _tensor(self.ctx, q, "q", f32, n, q.shape[1])
+        op, os_ = _tensor(self.ctx, out, "out", f32, n, q.shape[1])
+        rows = KvQueriesStruct(n, q.shape[1] // hs, qp, op, qs, os_, _tensor(self.ctx, seqs, "seqs", torch.int32, n)[0],
+                               _tensor(self.ctx, pos, "pos", torch.int32, n)[0], scale, window, sinks)
+        work = _workspace(self.ctx, self._work[layer], stream)
+        check(lib().g4_kv_attend(self.handle, layer, C.byref(rows), work.data_ptr(), work.numel(),
+                                 _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_attend")
+
+
+def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, tokens, finished=None,
+                pad_token: int = 0, stream=None) -> None:
+    """The `beams` best continuations of every group of `beams` rows of logits
+    [rows, vocab] (fp32): new_scores (fp32; may be scores), parents (int32 rows,
+    KvCache.fork's src) and tokens (int32), best first; -1 where too few remain.
+    finished (int32): rows whose one continuation is pad_token at their score."""
+    import torch
+
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    lp, ls = _tensor(ctx, logits, "logits", torch.float32, rows, vocab)
+    sp, _ = _tensor(ctx, scores, "scores", torch.float32, rows)
+    fp = None if finished is None else _tensor(ctx, finished, "finished", torch.int32, rows)[0]
+    np_, _ = _tensor(ctx, new_scores, "new_scores", torch.float32, rows)
+    pp, _ = _tensor(ctx, parents, "parents", torch.int32, rows)
+    tp, _ = _tensor(ctx, tokens, "tokens", torch.int32, rows)
+    work = _workspace(ctx, lib().g4_beam_select_workspace(rows, vocab, beams), stream)
+    check(lib().g4_beam_select(ctx.handle, lp, ls, vocab, sp, fp, rows, beams, pad_token, np_, pp, tp,
+                               work.data_ptr(), work.numel(), _stream(ctx, stream)), ctx.handle, "g4_beam_select")

@@ -322,6 +322,164 @@ void *g4_batch_stream(g4_batch *batch);
  * own sequences.  Q4_K experts; E divisible by W. */
 int g4_batch_expert_parallel(g4_batch *batch);
 
+/* ---------------- paged KV cache ----------------
+ * No reference counterpart: a LlamaState owns one contiguous cache
+ * (LlamaState.kt:38-77).  A g4_kv holds the K and V rows of many sequences in
+ * pages of page_size positions that sequences may share: forking a sequence
+ * (a beam, a common prompt) costs a row of the page table, not a copy.
+ *
+ * Device state, readable and writable by the caller through the accessors:
+ *   k, v    per layer [n_pages][n_kv_heads][page_size][head_size] of `type`
+ *   table   [n_seqs][ceil(max_positions / page_size)] page of every position
+ *           range, -1 where a sequence has none
+ *   lens    [n_seqs] positions a sequence has pages for
+ *   refs    [n_pages] sequences that hold a page (0: free)
+ * A new cache has no sequences (lens 0) and zeroed pages.
+ *
+ * The calls below read their arguments (sequence numbers, lengths, positions)
+ * from device memory, are asynchronous on `stream`, do not allocate and may be
+ * captured into a graph.  What they find wrong on the device (an entry out of
+ * range, no free page) they skip and record; g4_kv_check reports it.  Calls
+ * that change one cache (resize, fork, compact, copy_pages, append) must be
+ * ordered on the GPU, among each other and with the calls that read it;
+ * g4_kv_attend calls may overlap if each has its own work space. */
+typedef struct g4_kv g4_kv;
+typedef struct {
+  int n_layers;
+  const int *n_kv_heads;  /* [n_layers] 1..256 */
+  const int *head_size;   /* [n_layers] 8..512 in steps of 8 */
+  int type;               /* G4_TYPE_F32, G4_TYPE_F16 or G4_TYPE_BF16 */
+  int page_size;          /* positions: 16, 32, 64, 128 or 256 */
+  int n_pages;            /* 1..2^20 */
+  int n_seqs;             /* 1..4096 */
+  int max_positions;      /* of one sequence, 1..2^30 */
+} g4_kv_config;
+int g4_kv_create(g4_ctx *ctx, const g4_kv_config *cfg, g4_kv **out);
+/* The caller has waited for work that uses the cache. */
+int g4_kv_free(g4_kv *kv);
+void *g4_kv_k(const g4_kv *kv, int layer);
+void *g4_kv_v(const g4_kv *kv, int layer);
+int32_t *g4_kv_table(const g4_kv *kv);
+int32_t *g4_kv_lens(const g4_kv *kv);
+int32_t *g4_kv_refs(const g4_kv *kv);
+
+/* Sequence seqs_dev[i] gets pages for lens_dev[i] positions (0 frees it).
+ * Pages are taken lowest number first, in the order of the entries; pages
+ * given back in the call can be taken in it.  A sequence that grows into a
+ * partly filled last page that others share gets a copy of the filled part
+ * (all layers); the last of several such sequences in a call that is left as
+ * its only holder keeps the page.  Without enough free pages the call changes
+ * nothing.  Entries with seqs_dev[i] < 0 are padding; a sequence named twice
+ * counts once, by its first entry. n <= n_seqs. */
+int g4_kv_resize(g4_kv *kv, const int32_t *seqs_dev, const int32_t *lens_dev, int n, void *stream);
+/* Sequence dst_dev[i] gives back its pages and shares those of src_dev[i], all
+ * sources as they were before the call: a permutation reorders beams.  Entries
+ * with a negative number are padding (g4_beam_select's parents may be passed
+ * as they are). n <= n_seqs; destinations distinct (a repeated one counts by
+ * its first entry). */
+int g4_kv_fork(g4_kv *kv, const int32_t *src_dev, const int32_t *dst_dev, int n, void *stream);
+/* Moves live pages (refs > 0) to the front of the pool: with L of them, the
+ * k-th at or behind L goes to the k-th free page before L.  The table follows. */
+int g4_kv_compact(g4_kv *kv, void *stream);
+/* Copies whole pages, all layers, for callers that keep their own table.
+ * Destinations distinct and no sources; pairs with a negative number are
+ * padding. n <= n_pages. */
+int g4_kv_copy_pages(g4_kv *kv, const int32_t *src_dev, const int32_t *dst_dev, int n, void *stream);
+/* Waits for `stream`; G4_E_NOMEM after a resize that lacked pages, G4_E_DEVICE
+ * after skipped entries or rows, with the message; the record is cleared.
+ * free_pages may be NULL.  Not during a capture (G4_E_ARG). */
+int g4_kv_check(g4_kv *kv, int *free_pages, void *stream);
+
+/* Rotary positions (RotaryPositionEmbeddings.kt:8-53, applied as Llama.kt:83-103
+ * does for the half layout).  Element pairs of the first rot_dim elements of a
+ * head turn by position * f_m, f_m = theta^(-2m / rot_dim) / freq_factors[m];
+ * the rest of the head stays.  Scaling for long contexts: LINEAR divides f_m by
+ * factor; YARN divides it for the pairs that turn less than beta_slow times
+ * over original_ctx, leaves those that turn more than beta_fast times, and
+ * blends between, and multiplies cosine and sine by attn_factor (0: the default
+ * 0.1 ln(factor) + 1 for YARN, 1 otherwise). */
+#define G4_ROPE_HALF 0         /* pairs (m, m + rot_dim / 2) */
+#define G4_ROPE_INTERLEAVED 1  /* pairs (2m, 2m + 1) */
+#define G4_ROPE_UNSCALED 0
+#define G4_ROPE_LINEAR 1
+#define G4_ROPE_YARN 2
+typedef struct g4_rope g4_rope;
+typedef struct {
+  int head_size;             /* 8..512 in steps of 8 */
+  int rot_dim;               /* 4..head_size in steps of 4 */
+  int layout;
+  int scaling;
+  double theta;              /* above 1 */
+  double factor;
+  int original_ctx;          /* YARN */
+  double beta_fast, beta_slow;
+  double attn_factor;
+  const float *freq_factors; /* host [rot_dim / 2] (rope_freqs.weight) or NULL */
+} g4_rope_config;
+int g4_rope_create(g4_ctx *ctx, const g4_rope_config *cfg, g4_rope **out);
+int g4_rope_free(g4_rope *rope);
+/* out = x rotated, n_rows rows of n_heads heads at positions pos_dev[row];
+ * strides in floats between rows; out may be x.  Rows with a negative position
+ * are left as they were.  Rows 16-byte aligned. */
+int g4_rope_apply(const g4_rope *rope, const float *x_dev, int64_t x_stride, float *out_dev, int64_t out_stride,
+                  int n_heads, const int32_t *pos_dev, int n_rows, void *stream);
+
+/* New rows of a layer: row i is position pos[i] of sequence seqs[i].  Strides
+ * are floats between rows, so q, k and v may be columns of one fused
+ * projection; rows 16-byte aligned. */
+typedef struct {
+  int n_rows;
+  int n_heads;                    /* query heads; with q == NULL only K and V are stored */
+  const float *q, *k, *v;         /* device, [n_rows][heads * head_size] */
+  float *q_out;                   /* may be q */
+  int64_t q_stride, k_stride, v_stride, q_out_stride;
+  const int32_t *seqs, *pos;      /* device [n_rows] */
+  const float *q_norm, *k_norm;   /* device [head_size] RMS norm weights, or NULL: no norm (Llama.kt:39-59) */
+  int norm_v;                     /* the bare norm of V (Llama.kt:62-81) */
+  float eps;
+} g4_kv_rows;
+/* Llama.kt:157-195 for the rows: q_out = rotated, normed q; the normed, rotated
+ * K row and the (normed) V row go into their page, rounded to the cache's type
+ * (nearest).  rope NULL: no rotation.  A row with seqs[i] < 0 is padding and
+ * left as it was; (sequence, position) pairs distinct.  A position without a
+ * page, or in a page that sequences share, is not stored (g4_kv_check). */
+int g4_kv_append(g4_kv *kv, int layer, const g4_kv_rows *rows, const g4_rope *rope, void *stream);
+
+typedef struct {
+  int n_rows;
+  int n_heads;                /* a multiple of the layer's KV heads; query head h reads KV head h / (n_heads / n_kv) */
+  const float *q;             /* device [n_rows][n_heads * head_size] */
+  float *out;
+  int64_t q_stride, out_stride;
+  const int32_t *seqs, *pos;  /* device [n_rows] */
+  float scale;                /* of the scores (1 in Llama.kt:204-208) */
+  int window;                 /* positions t > pos - window are visible (0: all) */
+  int sinks;                  /* and positions t < sinks, however far back (with a window) */
+} g4_kv_queries;
+/* Attention of one new token per row over its sequence's pages (Llama.kt:197-218):
+ * softmax over the visible positions t <= pos[i], fp32 throughout.  Rows with
+ * seqs[i] < 0 are left as they were; a row with pos[i] < 0 sees nothing and
+ * gets zeros.  Visible cache entries must be finite; anything may lie in the
+ * others.  A visible position without a page counts as a row of zeros and is
+ * recorded (g4_kv_check).  `work`: g4_kv_attend_workspace bytes of the caller's, 16-byte
+ * aligned, one per call in flight. */
+size_t g4_kv_attend_workspace(const g4_kv *kv, int layer);
+int g4_kv_attend(g4_kv *kv, int layer, const g4_kv_queries *rows, void *work, size_t work_bytes, void *stream);
+
+/* Beam search's selection (no reference counterpart: Sampler.kt samples one
+ * sequence).  Rows [g * beams, (g + 1) * beams) of logits_dev [n_rows][stride]
+ * are group g; new_scores / parents / tokens [n_rows] get its `beams` best
+ * continuations, best first: score + logit - log sum exp(logits of the row).
+ * Ties go to the lower beam, then the lower token.  parents are row numbers
+ * (g4_kv_fork's src).  finished_dev (int32, NULL: none): a finished row has one
+ * continuation, pad_token at its own score.  Logits of -inf (masked tokens) and
+ * NaN are never chosen; where too few remain: score -inf, parent and token -1.
+ * new_scores may be scores.  beams <= 32; work as for g4_kv_attend. */
+size_t g4_beam_select_workspace(int n_rows, int vocab, int beams);
+int g4_beam_select(g4_ctx *ctx, const float *logits_dev, int64_t stride, int vocab, const float *scores_dev,
+                   const int32_t *finished_dev, int n_rows, int beams, int pad_token, float *new_scores_dev,
+                   int32_t *parents_dev, int32_t *tokens_dev, void *work, size_t work_bytes, void *stream);
+
 /* Router top-k alone on given logits (Llama.kt:273-293 + softmaxInPlace,
  * MutableFloatTensor.kt:54-59): probs_dev/idx_dev [n_tokens, k]. */
 int g4_moe_topk(g4_ctx *ctx, const float *logits_dev, int n_tokens, int n_expert, int k,
