@@ -27,21 +27,26 @@
 // positions change.  Runs that end inside an item leave (max, sum, O) partials
 // in the caller's work space; a second launch joins them in a fixed order.
 //
-// Warps are independent inside a run: each streams its own 16-position tiles
-// through a private ring in shared memory (cp.async, rows of masked positions
-// filled with zeros, so what lies there cannot reach the sums), keeps its
-// running maximum, sum and O^T in registers, and meets the CTA's other warps
-// once per item.
+// Inside a run one warp brings units in (TMA boxes of 16 positions x 128 bytes
+// of a head, swizzled so that fragment loads hit distinct banks; K and V of a
+// unit are two stages of one ring) and runs ahead over the ends of items, so
+// HBM stays busy while the others finish one. The other warps own 16 or 32
+// positions of every unit each, keep their running maximum, sum and O^T in
+// registers, and meet once per item. Positions that a row does not see are
+// left out of the scores by selection and their V rows are zeroed in shared
+// memory, so what lies there cannot reach the sums; boxes without a visible
+// position are not loaded.
 #include "g4_common.cuh"
 #include "g4_kv.h"
 
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
 namespace g4 {
 
 constexpr int kHeadBlock = 8;  // query heads per item: the mma's columns
 constexpr int kTile = 16;      // positions per warp and step: the mma's rows
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 256;
 
 struct AttendArgs {
   const float* q;
@@ -49,7 +54,6 @@ struct AttendArgs {
   long long q_stride, out_stride;
   const int32_t *seqs, *pos;
   int n_rows;
-  const uint8_t *kp, *vp;
   const int32_t* table;
   unsigned* flags;
   int n_seqs, max_pages, max_positions, page_shift, n_pages;
@@ -58,24 +62,32 @@ struct AttendArgs {
   float scale_log2;         // scale * log2(e): scores in powers of two
   int window, sinks;
   float* ws;                // [grid][2][kHeadBlock][hs + 2] partials: max, sum, O
+  int4* joins;              // [grid] the item a CTA begins and others go on with (x < 0: none)
 };
 
-// Shape of one instantiation: element type, padded head size, warps per CTA
-// and stages of a warp's ring (a stage holds 16 rows of K or of V).
+// Shape of one instantiation: element type, padded head size, warps that
+// compute, 16-position tiles per warp, stages of the ring (a stage holds a
+// unit's K or V). Two CTAs per SM share 192 KB of ring where a stage is 32 KB
+// or less; a wider head takes the SM's memory for one.
 template <int TYPE, int HSP>
 struct AttendShape {
   static constexpr int kElem = TYPE == F32 ? 4 : 2;
-  static constexpr int kStage = kTile * HSP * kElem;
-  static constexpr int kWarps = kStage > 16 * 1024 ? 2 : 4;
-  // two CTAs per SM where the ring allows it: 64 KB at 2 KB stages, 96 KB otherwise
-  static constexpr int kStages = kStage <= 2048 ? 8 : kStage <= 4096 ? 6 : 3;
+  static constexpr int kRow = HSP * kElem;  // bytes of a position, padded
+  static constexpr int kWarps = kRow > 1024 ? 2 : 4;
+  static constexpr int kTiles = kRow <= 256 ? 2 : 1;
+  static constexpr int kUnit = kWarps * kTiles * kTile;  // positions per unit
+  static constexpr int kStage = kUnit * kRow;
+  static constexpr int kStages = kStage <= 16384 ? 6 : 3;
+  static constexpr int kCtas = kStage <= 32768 ? 2 : 1;
   static constexpr int kParts = TYPE == F16 ? 2 : 3;
-  static constexpr int kCtas = kStage <= 8192 ? 2 : 1;
+  static constexpr int kBlocks = kRow / 128;              // 128-byte blocks of a row
+  static constexpr int kBlockBytes = kUnit * 128;         // one block of every position
+  static constexpr int kRing = kStages * kStage;
   static constexpr int kQBytes = kParts * HSP * kHeadBlock * 2;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kSmem = kRing + kQBytes;
-  static constexpr int kUnit = kWarps * kTile;  // positions per unit
-  static_assert(kWarps * kHeadBlock * HSP * 4 <= kRing, "the CTA's join reuses the ring");
+  static constexpr int kPitch = HSP + 4;                  // floats between heads where the warps meet
+  static constexpr int kMeet = kHeadBlock * kPitch * 4;   // shares the fragments' memory
+  static constexpr int kSmem = kRing + (kQBytes > kMeet ? kQBytes : kMeet);
+  static constexpr int kThreads = (kWarps + 1) * 32;
 };
 
 // The units of a row's visible positions: those of the first tokens, then
@@ -108,34 +120,17 @@ __device__ __forceinline__ long long run_start(long long total, int grid, int ct
   return total * cta / grid;
 }
 
-// All threads of the CTA; red holds 32 + 3 long longs.
+// All threads of the CTA. Up to a row per thread one scan gives both the
+// total and the place of w0; more rows are walked a second time.
 template <int THREADS>
 __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int grid, long long* red) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int NW = THREADS / 32;
-  long long sum = 0;
-  for (int r = tid; r < a.n_rows; r += THREADS) sum += row_units(a, r, unit).units;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();
-  if (lane == 0) red[warp] = sum;
-  __syncthreads();
-  long long total = 0;
-  for (int i = 0; i < NW; ++i) total += red[i];
-  total *= items;
-  // no more CTAs than units: the first ones get one unit each
-  const int used = (int)min((long long)grid, total);
   Run run;
-  run.total = total;
-  run.w0 = cta < used ? run_start(total, used, cta) : total;
-  run.w1 = cta < used ? run_start(total, used, cta + 1) : total;
-  run.row = 0;
-  run.row_start = 0;
-  if (run.w0 >= run.w1) return run;
-  long long before = 0;
-  for (int r0 = 0; r0 < a.n_rows; r0 += THREADS) {
-    const int r = r0 + tid;
-    long long mine = r < a.n_rows ? (long long)row_units(a, r, unit).units * items : 0, x = mine;
+  long long mine = 0, x = 0, before = 0, chunk = 0;
+  auto scan = [&](int r) {  // mine: units of row r; x: of the rows up to r in this chunk; chunk: of the chunk
+    mine = r < a.n_rows ? (long long)row_units(a, r, unit).units * items : 0;
+    x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, x, o);
@@ -144,23 +139,80 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
     __syncthreads();
     if (lane == 31) red[warp] = x;
     __syncthreads();
-    long long start = before + x - mine, chunk = 0;
+    chunk = 0;
     for (int i = 0; i < NW; ++i) {
-      if (i < warp) start += red[i];
+      if (i < warp) x += red[i];
       chunk += red[i];
     }
+  };
+  long long total = 0;
+  for (int r0 = 0; r0 < a.n_rows; r0 += THREADS) {
+    scan(r0 + tid);
+    total += chunk;
+  }
+  // no more CTAs than units: the first ones get one unit each
+  const int used = (int)min((long long)grid, total);
+  run.total = total;
+  run.w0 = cta < used ? run_start(total, used, cta) : total;
+  run.w1 = cta < used ? run_start(total, used, cta + 1) : total;
+  run.row = 0;
+  run.row_start = 0;
+  if (run.w0 >= run.w1) return run;
+  for (int r0 = 0; r0 < a.n_rows; r0 += THREADS) {
+    if (a.n_rows > THREADS) scan(r0 + tid);
+    const long long start = before + x - mine;
     if (mine > 0 && start <= run.w0 && run.w0 < start + mine) {
-      red[32] = r;
-      red[33] = start;
+      red[NW] = r0 + tid;
+      red[NW + 1] = start;
     }
     before += chunk;
     if (before > run.w0) break;
   }
   __syncthreads();
-  run.row = (int)red[32];
-  run.row_start = red[33];
+  run.row = (int)red[NW];
+  run.row_start = red[NW + 1];
   return run;
 }
+
+// A walk over a run: the part of one item after the other.
+struct Walk {
+  long long w, row_start;
+  int row, item, u0, n;  // units [u0, u0 + n) of the row's item
+  RowUnits ru;
+  bool loaded = false;
+  __device__ __forceinline__ void start(const Run& r) {
+    w = r.w0;
+    row = r.row;
+    row_start = r.row_start;
+    n = 0;
+  }
+  __device__ __forceinline__ bool next(const AttendArgs& a, const Run& r, int unit, int items) {
+    w += n;
+    if (w >= r.w1) return false;
+    if (!loaded) ru = row_units(a, row, unit);
+    loaded = true;
+    while (w >= row_start + (long long)ru.units * items) {
+      row_start += (long long)ru.units * items;
+      ru = row_units(a, ++row, unit);
+    }
+    item = (int)((w - row_start) / ru.units);
+    u0 = (int)(w - row_start - (long long)item * ru.units);
+    n = (int)min((long long)(ru.units - u0), r.w1 - w);
+    return true;
+  }
+  __device__ __forceinline__ int position(int j, int unit) const {  // first of unit u0 + j
+    const int u = u0 + j;
+    return (u < ru.sink_units ? u : ru.first_unit + u - ru.sink_units) * unit;
+  }
+  __device__ __forceinline__ bool seen(int t, int sinks) const { return t <= ru.pos && (t >= ru.low || t < sinks); }
+  __device__ __forceinline__ bool seen_tile(int t0, int sinks) const {
+    return t0 <= ru.pos && (t0 + kTile > ru.low || t0 < sinks);
+  }
+  // every position of the tile
+  __device__ __forceinline__ bool whole_tile(int t0, int sinks) const {
+    return t0 + kTile - 1 <= ru.pos && (t0 >= ru.low || t0 + kTile <= sinks);
+  }
+};
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -195,10 +247,18 @@ __device__ __forceinline__ float exp2_approx(float x) {  // relative error 2^-22
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 16 bytes global -> shared; zeros where !ok (nothing is read).
-__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// A box of 16 positions x 128 bytes of one head of a page.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page,
+                                        uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void bar_compute() {  // the computing warps
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
 // The next part of (x, y) in the mma's type, packed, and what it leaves of them.
@@ -218,32 +278,107 @@ __device__ __forceinline__ uint32_t take_part(float& x, float& y) {
   return u;
 }
 
-// Where 16-byte chunk c of row r lies in a stage: chunks change places within
-// a row so that the eight rows of a fragment load hit distinct banks.  fp32
-// fragments are pairs of chunks of rows {0..3}, {4..7}, {0,2,4,6} or
-// {1,3,5,7}: those sets get distinct even offsets.
-template <int TYPE>
-__device__ __forceinline__ int chunk_at(int r, int c) {
-  return TYPE == F32 ? c ^ (2 * (((r & 7) + ((r >> 2) & 1)) & 3)) : c ^ (r & 7);
+// Byte offset of 16-byte chunk c of position r in a stage: 128-byte blocks of
+// all positions one after the other, chunks swizzled within a row's block.
+template <int BLOCK>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)((c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 template <int TYPE, int HSP>
-__global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendShape<TYPE, HSP>::kCtas)
-    kv_attend_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<TYPE, HSP>::kCtas)
+    kv_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,
+                     const __grid_constant__ CUtensorMap v_map) {
   using S = AttendShape<TYPE, HSP>;
   constexpr bool HALF = TYPE == F16;
-  constexpr int NW = S::kWarps, NS = S::kStages, NP = S::kParts, KS = HSP / 16, CPR = HSP * S::kElem / 16;
-  extern __shared__ __align__(128) uint8_t smraw[];
-  __shared__ long long red[35];
+  constexpr int NW = S::kWarps, MT = S::kTiles, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
+  extern __shared__ __align__(1024) uint8_t smraw[];
+  __shared__ long long red[NW + 3];
   __shared__ float q_unscale[kHeadBlock];
   __shared__ float stat[NW][kHeadBlock][2];
+  __shared__ __align__(8) uint64_t full[NS], empty[NS];
+  __shared__ unsigned boxes[NS];  // the 16-position boxes of a stage that were loaded
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs;
-  uint8_t* ring = smraw + (size_t)warp * NS * S::kStage;
-  uint2* qf = reinterpret_cast<uint2*>(smraw + S::kRing);  // [part][k step][lane] B fragments
-  const uint32_t ring_u = smem_u32(ring);
-  const int items = a.n_kv * a.blocks, ks = (hs + 15) / 16, chunks = hs * S::kElem / 16;
+  const uint32_t ring = smem_u32(smraw);
+  uint2* qf = reinterpret_cast<uint2*>(smraw + S::kRing);     // [part][k step][lane] B fragments of q
+  float* meet = reinterpret_cast<float*>(smraw + S::kRing);   // [head][kPitch], between items
+  const int items = a.n_kv * a.blocks, ks = (hs + 15) / 16;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, NW);
+    }
+    fence_barrier_init();
+  }
   grid_dep_launch();
-  const Run run = find_run<NW * 32>(a, S::kUnit, items, blockIdx.x, gridDim.x, red);
+  const Run run = find_run<S::kThreads>(a, S::kUnit, items, blockIdx.x, gridDim.x, red);
+  __syncthreads();  // the barriers are set up (find_run may return before its last one)
+  Walk k;
+  k.start(run);
+  int stage = 0;
+  uint32_t phase = 0;
+  auto step = [&]() {
+    if (++stage == NS) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  };
+
+  if (warp == NW) {
+    // ---- the loading warp: lane b brings box b of every unit
+    const int nblk = (hs * S::kElem + 127) / 128;
+    int issued = 0;
+    bool ok = true;
+    while (ok && k.next(a, run, S::kUnit, items)) {
+      const int32_t* pages = a.table + (long long)k.ru.seq * a.max_pages;
+      const int kvh = k.item / a.blocks;
+      auto page_of = [&](int j) {
+        const int t = k.position(j, S::kUnit) + lane * kTile;
+        return lane < NW * MT && j < k.n && k.seen_tile(t, a.sinks) ? pages[t >> a.page_shift] : -2;
+      };
+      int page = page_of(0);
+      for (int j = 0; j < k.n && ok; ++j) {
+        const int after = page_of(j + 1);
+        const bool have = page >= 0 && page < a.n_pages;
+        if (page != -2 && !have) atomicOr(a.flags, KV_BAD_ROW);
+        const unsigned mask = __ballot_sync(0xffffffffu, have);
+        const int slot = (k.position(j, S::kUnit) + lane * kTile) & ((1 << a.page_shift) - 1);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (issued >= NS && !mbar_wait_bounded(empty + stage, phase ^ 1u)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            boxes[stage] = mask;
+            mbar_arrive_expect_tx(full + stage, (uint32_t)(__popc(mask) * nblk) * 2048u);
+          }
+          __syncwarp();
+          if (have) {
+            const uint32_t dst = ring + stage * S::kStage + lane * 2048;
+            for (int b = 0; b < nblk; ++b)
+              tma_box(dst + b * BLK, half ? &v_map : &k_map, b * (128 / S::kElem), slot, kvh, page, full + stage);
+          }
+          ++issued;
+          step();
+        }
+        page = after;
+      }
+    }
+    if (!ok) {  // the copies still in flight land before the CTA may leave
+      if (lane == 0) atomicOr(a.flags, KV_TIMEOUT);
+      for (int i = 0; i < NS && i < issued; ++i) {
+        if (--stage < 0) {
+          stage = NS - 1;
+          phase ^= 1u;
+        }
+        mbar_wait_bounded(full + stage, phase);
+      }
+    }
+    return;
+  }
+
+  // ---- the computing warps
   // rows that see nothing: zeros
   for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
     const int seq = a.seqs[r], pos = a.pos[r];
@@ -254,68 +389,23 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
       for (int i = tid; i < a.n_kv * a.group * hs; i += NW * 32) a.out[r * a.out_stride + i] = 0.f;
     }
   }
-  long long w = run.w0, row_start = run.row_start;
-  int row = run.row;
-  bool first = true;
-  while (w < run.w1) {
-    RowUnits ru = row_units(a, row, S::kUnit);
-    while (w >= row_start + (long long)ru.units * items) {
-      row_start += (long long)ru.units * items;
-      ru = row_units(a, ++row, S::kUnit);
+  bool dead = false;  // a wait expired: no more waits, the results are void
+  auto arrived = [&]() {
+    if (!dead && !mbar_wait_bounded(full + stage, phase)) {
+      dead = true;
+      if (lane == 0) atomicOr(a.flags, KV_TIMEOUT);
     }
-    const int item = (int)((w - row_start) / ru.units);
-    const int u0 = (int)((w - row_start) - (long long)item * ru.units);
-    const int u1 = (int)min((long long)ru.units, u0 + (run.w1 - w));
-    const int kvh = item / a.blocks, h0 = (item - kvh * a.blocks) * kHeadBlock, nh = min(kHeadBlock, a.group - h0);
-    const float* q = a.q + row * a.q_stride + (long long)(kvh * a.group + h0) * hs;
-    const int32_t* pages = a.table + (long long)ru.seq * a.max_pages;
-    const int n = u1 - u0;
-
-    // ---- K and V tiles on their way before anything else
-    auto tile_pos = [&](int j) {  // first position of this warp's tile of unit u0 + j
-      const int u = u0 + j;
-      return (u < ru.sink_units ? u : ru.first_unit + u - ru.sink_units) * S::kUnit + warp * kTile;
-    };
-    auto seen = [&](int t) { return t <= ru.pos && (t >= ru.low || t < a.sinks); };
-    auto seen_tile = [&](int t0) { return t0 <= ru.pos && (t0 + kTile > ru.low || t0 < a.sinks); };
-    auto tile_page = [&](int j) {  // -1: no position of the tile is visible, or its page is missing
-      const int t = tile_pos(j);
-      return j < n && seen_tile(t) ? pages[t >> a.page_shift] : -1;
-    };
-    auto issue = [&](int j, int page, bool is_v, int stage) {
-      if (j < n) {
-        const int t0 = tile_pos(j);
-        const bool have = (unsigned)page < (unsigned)a.n_pages;
-        if (!have && seen_tile(t0) && lane == 0) atomicOr(a.flags, KV_BAD_ROW);
-        const uint8_t* src = (is_v ? a.vp : a.kp) +
-                             (((((long long)(have ? page : 0) * a.n_kv + kvh) << a.page_shift) +
-                               (t0 & ((1 << a.page_shift) - 1))) * hs) * S::kElem;
-        const uint32_t dst = ring_u + stage * S::kStage;
-#pragma unroll
-        for (int i = 0; i < kTile * CPR / 32; ++i) {
-          const int e = lane + 32 * i, r = e / CPR, c = e % CPR;
-          // chunks behind the head's end are zeros up to the next k step
-          if (c < ks * S::kElem)
-            cp16_or_zero(dst + (uint32_t)(r * CPR + chunk_at<TYPE>(r, c)) * 16u,
-                         src + ((long long)r * chunks + (c < chunks ? c : 0)) * 16, have && seen(t0 + r) && c < chunks);
-        }
-      }
-      cp_commit();
-    };
-    // half tile h is K (even) or V (odd) of tile h / 2; NS - 1 of them in flight
-    int next = 0, next_stage = 0;
-    int page_a = tile_page(0), page_b = tile_page(1);  // pages of tiles next / 2 and the one behind it
-    auto issue_next = [&]() {
-      issue(next >> 1, page_a, next & 1, next_stage);
-      if (next & 1) {
-        page_a = page_b;
-        page_b = tile_page((next >> 1) + 2);
-      }
-      ++next;
-      next_stage = next_stage + 1 == NS ? 0 : next_stage + 1;
-    };
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) issue_next();
+  };
+  auto release = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + stage);
+    step();
+  };
+  bool first = true;
+  int4 pending = make_int4(-1, 0, 0, 0);  // the item that goes on in the next CTA
+  while (k.next(a, run, S::kUnit, items)) {
+    const int kvh = k.item / a.blocks, h0 = (k.item - kvh * a.blocks) * kHeadBlock, nh = min(kHeadBlock, a.group - h0);
+    const float* q = a.q + k.row * a.q_stride + (long long)(kvh * a.group + h0) * hs;
 
     // ---- q of the block's heads as B fragments: k = dims, n = heads
     if (HALF) {  // a power of two per head brings its largest element to 2^13..2^14
@@ -329,7 +419,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
         if (m > 0.f && m < INFINITY) frexpf(m, &e);
         if (lane == 0) q_unscale[h] = ldexpf(1.f, max(-100, min(100, e - 14)));
       }
-      __syncthreads();
+      bar_compute<NW * 32>();
     }
     for (int i = tid; i < ks * 32; i += NW * 32) {
       const int kk = i >> 5, h = (i & 31) >> 2, d = kk * 16 + 2 * (i & 3);
@@ -350,47 +440,61 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
         qf[(p * KS + kk) * 32 + (i & 31)] = b;
       }
     }
-    __syncthreads();
+    bar_compute<NW * 32>();
     float sc[2];  // score factors of this thread's two heads
 #pragma unroll
     for (int j = 0; j < 2; ++j) sc[j] = a.scale_log2 * (HALF ? q_unscale[2 * (lane & 3) + j] : 1.f);
 
-    // ---- the warp's tiles
+    // ---- the warp's tiles of every unit
     float o[KS][4];
 #pragma unroll
     for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int stage = 0;
-    for (int j = 0; j < n; ++j) {
-      const int t0 = tile_pos(j);
-      // K
-      cp_wait<NS - 2>();
-      __syncwarp();
-      issue_next();
-      uint32_t pf[NP][2];
+    for (int j = 0; j < k.n; ++j) {
+      const int t0 = k.position(j, S::kUnit) + warp * MT * kTile;  // the warp's first position
+      arrived();
+      const unsigned mine = (boxes[stage] >> (warp * MT)) & ((1u << MT) - 1u);
+      if (mine == 0) {  // nothing visible here
+        release();
+        arrived();
+        release();
+        continue;
+      }
+      uint32_t pf[MT][NP][2];
+      bool partial = false;
       {
-        float s[NP][4];
+        float s[MT][NP][4];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) s[p][0] = s[p][1] = s[p][2] = s[p][3] = 0.f;
-        const uint32_t kt = ring_u + stage * S::kStage;
-        const uint8_t* kg = ring + stage * S::kStage;
+        for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-          if (kk < ks) {
-            if (TYPE != F32) {
+          for (int p = 0; p < NP; ++p) s[t][p][0] = s[t][p][1] = s[t][p][2] = s[t][p][3] = 0.f;
+        const uint32_t kt = ring + stage * S::kStage;
+        const uint8_t* kg = smraw + stage * S::kStage;
+        if (TYPE != F32) {
+#pragma unroll 4
+          for (int kk = 0; kk < ks; ++kk) {
+            uint2 b[NP];
+#pragma unroll
+            for (int p = 0; p < NP; ++p) b[p] = qf[(p * KS + kk) * 32 + lane];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
               uint32_t ka[4];
-              ldsm4(ka, kt + (uint32_t)((lane & 15) * CPR + chunk_at<TYPE>(lane & 15, 2 * kk + (lane >> 4))) * 16u);
+              ldsm4(ka, kt + chunk_at<BLK>((warp * MT + t) * kTile + (lane & 15), 2 * kk + (lane >> 4)));
 #pragma unroll
-              for (int p = 0; p < NP; ++p) {
-                const uint2 b = qf[(p * KS + kk) * 32 + lane];
-                mma16816<HALF>(s[p], ka, b.x, b.y);
-              }
-            } else {
+              for (int p = 0; p < NP; ++p) mma16816<HALF>(s[t][p], ka, b[p].x, b[p].y);
+            }
+          }
+        } else {
+#pragma unroll 2
+          for (int kk = 0; kk < ks; ++kk) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
               float x[8];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {  // (row, row + 8) x (col, col + 8)
-                const int r = (lane >> 2) + (i & 1) * 8, c = kk * 4 + (i >> 1) * 2 + ((lane & 3) >> 1);
-                const float2 v = *reinterpret_cast<const float2*>(kg + (r * CPR + chunk_at<TYPE>(r, c)) * 16 + (lane & 1) * 8);
+                const int r = (warp * MT + t) * kTile + (lane >> 2) + (i & 1) * 8;
+                const int c = kk * 4 + (i >> 1) * 2 + ((lane & 3) >> 1);
+                const float2 v = *reinterpret_cast<const float2*>(kg + chunk_at<BLK>(r, c) + (lane & 1) * 8);
                 x[2 * i] = v.x;
                 x[2 * i + 1] = v.y;
               }
@@ -403,28 +507,34 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
               for (int p = 0; p < NP; ++p) {  // products of parts i + p <= 2
                 const uint2 b = qf[(p * KS + kk) * 32 + lane];
 #pragma unroll
-                for (int i = 0; i < 3 - p; ++i) mma16816<false>(s[i], ka[i], b.x, b.y);
+                for (int i = 0; i < 3 - p; ++i) mma16816<false>(s[t][i], ka[i], b.x, b.y);
               }
             }
           }
         }
+        release();
         // scores: rows t0 + lane / 4 (+ 8), columns heads 2 (lane % 4) (+ 1)
-        const bool s0 = seen(t0 + (lane >> 2)), s1 = seen(t0 + (lane >> 2) + 8);
-        float x[4];
+        float x[MT][4], mn[2] = {m[0], m[1]};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = s[NP - 1][i];
+        for (int t = 0; t < MT; ++t) {
+          const int tt = t0 + t * kTile;
+          const bool have = (mine >> t) & 1u, whole = have && k.whole_tile(tt, a.sinks);
+          partial |= !whole;
 #pragma unroll
-          for (int p = NP - 2; p >= 0; --p) v += s[p][i];
-          x[i] = ((i >> 1) ? s1 : s0) ? v * sc[i & 1] : -INFINITY;
+          for (int i = 0; i < 4; ++i) {
+            float v = s[t][NP - 1][i];
+#pragma unroll
+            for (int p = NP - 2; p >= 0; --p) v += s[t][p][i];
+            const bool vis = whole || (have && k.seen(tt + (lane >> 2) + (i >> 1) * 8, a.sinks));
+            x[t][i] = vis ? v * sc[i & 1] : -INFINITY;
+          }
+          mn[0] = fmaxf(mn[0], fmaxf(x[t][0], x[t][2]));
+          mn[1] = fmaxf(mn[1], fmaxf(x[t][1], x[t][3]));
         }
-        float mn[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mn[h] = fmaxf(x[h], x[h + 2]);
-#pragma unroll
-          for (int b = 4; b < 32; b <<= 1) mn[h] = fmaxf(mn[h], __shfl_xor_sync(0xffffffffu, mn[h], b));
-          mn[h] = fmaxf(mn[h], m[h]);
+        for (int b = 4; b < 32; b <<= 1) {
+          mn[0] = fmaxf(mn[0], __shfl_xor_sync(0xffffffffu, mn[0], b));
+          mn[1] = fmaxf(mn[1], __shfl_xor_sync(0xffffffffu, mn[1], b));
         }
         if (__any_sync(0xffffffffu, mn[0] != m[0] || mn[1] != m[1])) {
           float f[2];
@@ -443,61 +553,75 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
           }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // f16 parts: p up to 2^8, so that the second part of a small p stays normal
-          const float mm = m[i & 1] == -INFINITY ? 0.f : m[i & 1];
-          x[i] = exp2_approx(x[i] - mm + (HALF ? 8.f : 0.f));
-          l[i & 1] += x[i];
-        }
+        for (int t = 0; t < MT; ++t) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          pf[p][0] = transpose8(take_part<HALF>(x[0], x[1]));
-          pf[p][1] = transpose8(take_part<HALF>(x[2], x[3]));
+          for (int i = 0; i < 4; ++i) {
+            // f16 parts: p up to 2^8, so that the second part of a small p stays normal
+            const float mm = m[i & 1] == -INFINITY ? 0.f : m[i & 1];
+            x[t][i] = exp2_approx(x[t][i] - mm + (HALF ? 8.f : 0.f));
+            l[i & 1] += x[t][i];
+          }
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            pf[t][p][0] = transpose8(take_part<HALF>(x[t][0], x[t][1]));
+            pf[t][p][1] = transpose8(take_part<HALF>(x[t][2], x[t][3]));
+          }
         }
       }
-      stage = stage + 1 == NS ? 0 : stage + 1;
-      // V
-      cp_wait<NS - 2>();
-      __syncwarp();
-      issue_next();
+      arrived();
       {
-        const uint32_t vt = ring_u + stage * S::kStage;
-        const uint8_t* vg = ring + stage * S::kStage;
+        const uint32_t vt = ring + stage * S::kStage;
+        const uint8_t* vg = smraw + stage * S::kStage;
+        if (partial) {  // V rows that are not seen become zeros
+          for (int e = lane; e < MT * kTile * 8; e += 32) {
+            const int r = e >> 3, t = t0 + r;
+            if (!((mine >> (r / kTile)) & 1u) || !k.seen(t, a.sinks))
+              for (int b = 0; b < (ks * S::kElem + 7) / 8; ++b)
+                *reinterpret_cast<uint4*>(smraw + stage * S::kStage + b * BLK + (warp * MT * kTile + r) * 128 + (e & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+          // ordered before the stage's next load, which another proxy writes
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           if (i < ks) {
-            if (TYPE != F32) {
-              uint32_t va[4];
-              const int r = (lane & 7) + (lane >> 4) * 8;
-              ldsm4_t(va, vt + (uint32_t)(r * CPR + chunk_at<TYPE>(r, 2 * i + ((lane >> 3) & 1))) * 16u);
 #pragma unroll
-              for (int p = 0; p < NP; ++p) mma16816<HALF>(o[i], va, pf[p][0], pf[p][1]);
-            } else {
-              // V[pos 2 (lane % 4) + {0, 1} (+ 8)][dim lane / 4 (+ 8)]: registers (dim), (dim + 8), then pos + 8
-              float x[8];
+            for (int t = 0; t < MT; ++t) {
+              if (TYPE != F32) {
+                uint32_t va[4];
+                const int r = (warp * MT + t) * kTile + (lane & 7) + (lane >> 4) * 8;
+                ldsm4_t(va, vt + chunk_at<BLK>(r, 2 * i + ((lane >> 3) & 1)));
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int r = 2 * (lane & 3) + (e & 1) + (e >> 2) * 8, d = i * 16 + (lane >> 2) + ((e >> 1) & 1) * 8;
-                x[e] = *reinterpret_cast<const float*>(vg + (r * CPR + chunk_at<TYPE>(r, d >> 2)) * 16 + (d & 3) * 4);
+                for (int p = NP - 1; p >= 0; --p) mma16816<HALF>(o[i], va, pf[t][p][0], pf[t][p][1]);
+              } else {
+                // V[pos 2 (lane % 4) + {0, 1} (+ 8)][dim lane / 4 (+ 8)]: registers (dim), (dim + 8), then pos + 8
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const int r = (warp * MT + t) * kTile + 2 * (lane & 3) + (e & 1) + (e >> 2) * 8;
+                  const int d = i * 16 + (lane >> 2) + ((e >> 1) & 1) * 8;
+                  x[e] = *reinterpret_cast<const float*>(vg + chunk_at<BLK>(r, d >> 2) + (d & 3) * 4);
+                }
+                uint32_t va[3][4];
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) va[p][e] = take_part<false>(x[2 * e], x[2 * e + 1]);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                  for (int e = 2 - p; e >= 0; --e) mma16816<false>(o[i], va[e], pf[t][p][0], pf[t][p][1]);
               }
-              uint32_t va[3][4];
-#pragma unroll
-              for (int p = 0; p < 3; ++p)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) va[p][e] = take_part<false>(x[2 * e], x[2 * e + 1]);
-#pragma unroll
-              for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                for (int e = 2 - p; e >= 0; --e) mma16816<false>(o[i], va[e], pf[p][0], pf[p][1]);
             }
           }
         }
       }
-      stage = stage + 1 == NS ? 0 : stage + 1;
+      release();
     }
-    cp_wait<0>();
 
-    // ---- the CTA's warps meet: common maximum, sums, O
+    // ---- the warps meet: common maximum, sums, O (added in the warps' order)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -507,36 +631,40 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
         stat[warp][2 * lane + h][1] = l[h];
       }
     }
-    __syncthreads();  // also: every warp has left the ring
-    float* part = reinterpret_cast<float*>(smraw);  // [NW][kHeadBlock][HSP]
+    bar_compute<NW * 32>();  // also: every warp has read its last q fragment
+    float f[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int head = 2 * (lane & 3) + h;
       float M = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][head][0]);
-      const float f = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - M);
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        float* at = part + (warp * kHeadBlock + head) * HSP + i * 16 + (lane >> 2);
-        at[0] = o[i][h] * f;
-        at[8] = o[i][2 + h] * f;
-      }
+      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][2 * (lane & 3) + h][0]);
+      f[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - M);
     }
-    __syncthreads();
-    const bool whole = u0 == 0 && u1 == ru.units;
+#pragma unroll 1
+    for (int w = 0; w < NW; ++w) {
+      if (w == warp) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            float* at = meet + (2 * (lane & 3) + h) * S::kPitch + i * 16 + (lane >> 2);
+            at[0] = (w ? at[0] : 0.f) + o[i][h] * f[h];
+            at[8] = (w ? at[8] : 0.f) + o[i][2 + h] * f[h];
+          }
+      }
+      bar_compute<NW * 32>();
+    }
+    const bool whole = k.u0 == 0 && k.n == k.ru.units;
     for (int e = tid; e < nh * hs; e += NW * 32) {
       const int h = e / hs, d = e - h * hs;
-      float M = -INFINITY, L = 0.f, acc = 0.f;
+      float M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][h][0]);
 #pragma unroll
-      for (int i = 0; i < NW; ++i) {
-        L += stat[i][h][0] == -INFINITY ? 0.f : exp2_approx(stat[i][h][0] - M) * stat[i][h][1];
-        acc += part[(i * kHeadBlock + h) * HSP + d];
-      }
+      for (int i = 0; i < NW; ++i) L += stat[i][h][0] == -INFINITY ? 0.f : exp2_approx(stat[i][h][0] - M) * stat[i][h][1];
+      const float acc = meet[h * S::kPitch + d];
       if (whole) {
-        a.out[row * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d] = L > 0.f ? acc / L : 0.f;
+        a.out[k.row * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d] = L > 0.f ? acc / L : 0.f;
       } else {
         float* ws = a.ws + ((long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock + h) * (hs + 2);
         if (d == 0) {
@@ -546,45 +674,35 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kWarps * 32, AttendSha
         ws[2 + d] = acc;
       }
     }
-    __syncthreads();  // the ring, the fragments and the statistics are free again
-    w += n;
+    if (!whole && k.u0 == 0) pending = make_int4(k.row, k.item, first ? 0 : 1, 0);
+    if (pending.x >= 0 && pending.w == 0) {  // the CTA of the item's last unit
+      const int used = (int)min((long long)gridDim.x, run.total);
+      const long long end = k.w + k.ru.units;
+      int last = blockIdx.x + 1;
+      while (run_start(run.total, used, last + 1) < end) ++last;
+      pending.w = last;
+    }
+    bar_compute<NW * 32>();  // the meeting place and the statistics are free again
     first = false;
   }
+  if (tid == 0) a.joins[blockIdx.x] = pending;
 }
 
 // Joins the partials of items that span CTAs: block (c, h) takes head h of the
 // item that starts in CTA c and does not end there.
-__global__ void __launch_bounds__(kJoinThreads) kv_attend_join_kernel(const __grid_constant__ AttendArgs a, int unit,
-                                                                      int grid) {
-  __shared__ long long red[35];
+__global__ void __launch_bounds__(kJoinThreads) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
   __shared__ float wsum[kJoinThreads / 32];
   __shared__ float acc_s[kJoinThreads / 32][kKvMaxHeadSize];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, c = blockIdx.x, h = blockIdx.y;
   constexpr int NW = kJoinThreads / 32;
-  const int items = a.n_kv * a.blocks;
-  const Run run = find_run<kJoinThreads>(a, unit, items, c, grid, red);
-  if (run.w0 >= run.w1) return;
-  // the item of the run's last unit
-  long long row_start = run.row_start;
-  int row = run.row;
-  RowUnits ru = row_units(a, row, unit);
-  while (run.w1 - 1 >= row_start + (long long)ru.units * items) {
-    row_start += (long long)ru.units * items;
-    ru = row_units(a, ++row, unit);
-  }
-  const int item = (int)((run.w1 - 1 - row_start) / ru.units);
-  const long long i0 = row_start + (long long)item * ru.units, i1 = i0 + ru.units;
-  if (i0 < run.w0 || i1 <= run.w1) return;
-  const int kvh = item / a.blocks, h0 = (item - kvh * a.blocks) * kHeadBlock;
-  if (h >= min(kHeadBlock, a.group - h0)) return;
-  const int used = (int)min((long long)grid, run.total);
-  int last = c + 1;
-  while (run_start(run.total, used, last + 1) < i1) ++last;
-  const int own_slot = i0 == run.w0 ? 0 : 1;
-  auto partial = [&](int i) {  // of CTA i
-    return a.ws + ((long long)(i * 2 + (i == c ? own_slot : 0)) * kHeadBlock + h) * (hs + 2);
-  };
   grid_dep_wait();
+  const int4 j = __ldcg(a.joins + c);  // row, item, slot in c, last CTA
+  if (j.x < 0) return;
+  const int kvh = j.y / a.blocks, h0 = (j.y - kvh * a.blocks) * kHeadBlock, last = j.w;
+  if (h >= min(kHeadBlock, a.group - h0)) return;
+  auto partial = [&](int i) {  // of CTA i
+    return a.ws + ((long long)(i * 2 + (i == c ? j.z : 0)) * kHeadBlock + h) * (hs + 2);
+  };
   float M = -INFINITY;
   for (int i = c + lane; i <= last; i += 32) M = fmaxf(M, __ldcg(partial(i)));
 #pragma unroll
@@ -623,20 +741,20 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attend_join_kernel(const __gr
       s += acc_s[i][d];
       t += wsum[i];
     }
-    a.out[row * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d] = t > 0.f ? s / t : 0.f;
+    a.out[j.x * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d] = t > 0.f ? s / t : 0.f;
   }
 }
 
-using AttendFn = void (*)(const AttendArgs);
+using AttendFn = void (*)(const AttendArgs, const CUtensorMap, const CUtensorMap);
 struct AttendPlan {
   AttendFn fn;
-  int threads, smem, unit, ctas;
+  int threads, smem, ctas;
 };
 
 template <int TYPE, int HSP>
 static AttendPlan attend_plan_s() {
   using S = AttendShape<TYPE, HSP>;
-  return AttendPlan{kv_attend_kernel<TYPE, HSP>, S::kWarps * 32, S::kSmem, S::kUnit, S::kCtas};
+  return AttendPlan{kv_attend_kernel<TYPE, HSP>, S::kThreads, S::kSmem, S::kCtas};
 }
 template <int TYPE>
 static AttendPlan attend_plan_t(int hs) {
@@ -649,8 +767,29 @@ static AttendPlan attend_plan(int type, int hs) {
   return type == F32 ? attend_plan_t<F32>(hs) : type == F16 ? attend_plan_t<F16>(hs) : attend_plan_t<BF16>(hs);
 }
 
-int kv_attend_prepare(const g4_kv* kv) {
-  cudaError_t e = cudaSuccess;
+// 16 positions x 128 bytes of one head of a page, zeros beyond the head's end.
+static bool make_map(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* map, const g4_kv* kv, int layer, void* base) {
+  const cuuint64_t hs = kv->hs[layer], ps = kv->page_size, nkv = kv->n_kv[layer], e = kv->elem;
+  const cuuint64_t dims[4] = {hs, ps, nkv, (cuuint64_t)kv->n_pages};
+  const cuuint64_t strides[3] = {hs * e, ps * hs * e, nkv * ps * hs * e};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / e), kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = kv->type == G4_TYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : kv->type == G4_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(map, type, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int kv_attend_prepare(g4_kv* kv) {
+  void* entry = nullptr;
+  cudaDriverEntryPointQueryResult q{};
+  cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &q);
+  if (!e && (q != cudaDriverEntryPointSuccess || !entry)) e = cudaErrorNotSupported;
+  for (int l = 0; l < kv->n_layers && !e; ++l) {
+    auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(entry);
+    if (!make_map(encode, &kv->k_map[l], kv, l, kv->k[l]) || !make_map(encode, &kv->v_map[l], kv, l, kv->v[l]))
+      e = cudaErrorInvalidValue;
+  }
   for (int l = 0; l < kv->n_layers && !e; ++l) {
     const AttendPlan p = attend_plan(kv->type, kv->hs[l]);
     e = cudaFuncSetAttribute(p.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, p.smem);
@@ -669,7 +808,8 @@ extern "C" {
 size_t g4_kv_attend_workspace(const g4_kv* kv, int layer) {
   if (!kv || layer < 0 || layer >= kv->n_layers) return 0;
   const AttendPlan p = attend_plan(kv->type, kv->hs[layer]);
-  return (size_t)kv->ctx->dev.sms * p.ctas * 2 * kHeadBlock * (kv->hs[layer] + 2) * sizeof(float);
+  const size_t grid = (size_t)kv->ctx->dev.sms * p.ctas;
+  return grid * (sizeof(int4) + 2 * kHeadBlock * (kv->hs[layer] + 2) * sizeof(float));
 }
 
 int g4_kv_attend(g4_kv* kv, int layer, const g4_kv_queries* rows, void* work, size_t work_bytes, void* stream) {
@@ -706,8 +846,6 @@ int g4_kv_attend(g4_kv* kv, int layer, const g4_kv_queries* rows, void* work, si
   a.seqs = rows->seqs;
   a.pos = rows->pos;
   a.n_rows = n;
-  a.kp = kv->k[layer];
-  a.vp = kv->v[layer];
   a.table = kv->table;
   a.flags = kv->flags;
   a.n_seqs = kv->n_seqs;
@@ -722,15 +860,16 @@ int g4_kv_attend(g4_kv* kv, int layer, const g4_kv_queries* rows, void* work, si
   a.scale_log2 = rows->scale * 1.4426950408889634f;
   a.window = rows->window;
   a.sinks = rows->window > 0 ? rows->sinks : 0;
-  a.ws = static_cast<float*>(work);
   const AttendPlan p = attend_plan(kv->type, hs);
   const int grid = c->dev.sms * p.ctas;
+  a.joins = static_cast<int4*>(work);
+  a.ws = reinterpret_cast<float*>(a.joins + grid);
   cudaStream_t st = (cudaStream_t)stream;
-  p.fn<<<grid, p.threads, p.smem, st>>>(a);
+  p.fn<<<grid, p.threads, p.smem, st>>>(a, kv->k_map[layer], kv->v_map[layer]);
   cudaError_t e = cudaGetLastError();
   if (!e)
     e = launch_after(kv_attend_join_kernel, dim3(grid, a.group < kHeadBlock ? a.group : kHeadBlock), dim3(kJoinThreads),
-                     0, st, a, p.unit, grid);
+                     0, st, a);
   return e ? c->cuda_fail(e, "g4_kv_attend") : 0;
 }
 

@@ -424,6 +424,8 @@ int g4_kv_create(g4_ctx* c, const g4_kv_config* cfg, g4_kv** out) {
     kv->hs.assign(cfg->head_size, cfg->head_size + cfg->n_layers);
     kv->k.resize(cfg->n_layers);
     kv->v.resize(cfg->n_layers);
+    kv->k_map.resize(cfg->n_layers);
+    kv->v_map.resize(cfg->n_layers);
     for (int l = 0; l < cfg->n_layers; ++l)
       bytes += 2 * (((uint64_t)kv->n_pages * kv->n_kv[l] * ps * kv->hs[l] * kv->elem + 255) / 256 * 256);
     size_t n_strips = 0;
@@ -603,10 +605,11 @@ int g4_kv_check(g4_kv* kv, int* free_pages, void* stream) {
   if (e) return c->cuda_fail(e, "g4_kv_check");
   if (free_pages) *free_pages = (int)h[1];
   if (!h[0]) return 0;
-  c->set_err("g4_kv_check:%s%s%s%s", h[0] & KV_NO_PAGES ? " not enough free pages (the resize changed nothing);" : "",
+  c->set_err("g4_kv_check:%s%s%s%s%s", h[0] & KV_NO_PAGES ? " not enough free pages (the resize changed nothing);" : "",
              h[0] & KV_BAD_ENTRY ? " an entry's sequence, length or page is out of range or named twice;" : "",
              h[0] & KV_NOT_STORED ? " an appended position has no page or lies in a shared one;" : "",
-             h[0] & KV_BAD_ROW ? " a row's sequence or position is out of range or sees a position without a page;" : "");
+             h[0] & KV_BAD_ROW ? " a row's sequence or position is out of range or sees a position without a page;" : "",
+             h[0] & KV_TIMEOUT ? " a bounded wait expired inside a kernel;" : "");
   return h[0] == KV_NO_PAGES ? G4_E_NOMEM : G4_E_DEVICE;
 }
 

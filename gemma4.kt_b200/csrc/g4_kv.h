@@ -4,6 +4,8 @@
 #include "g4.h"
 #include "g4_ctx.h"
 
+#include <cuda.h>
+
 #include <vector>
 
 constexpr int kKvMaxSeqs = 4096;
@@ -15,6 +17,7 @@ enum KvFlag : unsigned {
   KV_NO_PAGES = 1u,  // g4_kv_resize: fewer free pages than the call needs
   KV_BAD_ENTRY = 2u, // a sequence, length or page out of range, or a sequence twice in one call
   KV_NOT_STORED = 4u,// g4_kv_append: position without a page, or in a page that sequences share
+  KV_TIMEOUT = 16u,  // a bounded wait inside a kernel expired
   KV_BAD_ROW = 8u,   // g4_kv_attend / g4_kv_append: sequence or position out of range, or a visible position without a page
 };
 
@@ -38,6 +41,7 @@ struct g4_kv {
   int n_strips = 0;
   std::vector<int> n_kv, hs;
   std::vector<uint8_t*> k, v;  // per layer [n_pages][n_kv][page_size][hs]
+  std::vector<CUtensorMap> k_map, v_map;  // per layer: 16 positions x 128 bytes of a head in a page, 128-byte swizzle
   uint8_t* pool = nullptr;
   uint8_t* meta = nullptr;     // everything below, one allocation
   int32_t *table = nullptr, *lens = nullptr, *refs = nullptr;
@@ -84,7 +88,7 @@ cudaError_t launch_after(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t s
 
 // Set-up of the kernels of one translation unit on the current device (loads
 // them, so that a first call may be captured); cudaError_t as int.
-int kv_attend_prepare(const g4_kv* kv);
+int kv_attend_prepare(g4_kv* kv);
 int rope_prepare();
 int beam_prepare();
 

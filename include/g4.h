@@ -460,8 +460,8 @@ typedef struct {
  * softmax over the visible positions t <= pos[i], fp32 throughout.  Rows with
  * seqs[i] < 0 are left as they were; a row with pos[i] < 0 sees nothing and
  * gets zeros.  Visible cache entries must be finite; anything may lie in the
- * others.  A visible position without a page counts as a row of zeros and is
- * recorded (g4_kv_check).  `work`: g4_kv_attend_workspace bytes of the caller's, 16-byte
+ * others.  A visible position without a page is left out and recorded
+ * (g4_kv_check).  `work`: g4_kv_attend_workspace bytes of the caller's, 16-byte
  * aligned, one per call in flight. */
 size_t g4_kv_attend_workspace(const g4_kv *kv, int layer);
 int g4_kv_attend(g4_kv *kv, int layer, const g4_kv_queries *rows, void *work, size_t work_bytes, void *stream);
