@@ -47,6 +47,7 @@ namespace g4 {
 constexpr int kHeadBlock = 8;  // query heads per item: the mma's columns
 constexpr int kTile = 16;      // positions per warp and step: the mma's rows
 constexpr int kJoinThreads = 256;
+constexpr int kItemUnits = 1;
 
 struct AttendArgs {
   const float* q;
@@ -96,10 +97,10 @@ struct RowUnits {
   int seq, pos, sink_units, first_unit, units, low;  // low: first position of the window
 };
 
-__device__ __forceinline__ RowUnits row_units(const AttendArgs& a, int row, int unit) {
+__device__ __forceinline__ RowUnits row_units(const AttendArgs& a, int seq, int pos, int unit) {
   RowUnits r;
-  r.seq = a.seqs[row];
-  r.pos = a.pos[row];
+  r.seq = seq;
+  r.pos = pos;
   r.units = r.sink_units = r.first_unit = r.low = 0;
   if (r.seq < 0 || r.seq >= a.n_seqs || r.pos < 0 || r.pos >= a.max_positions) return r;
   if (a.window > 0) r.low = max(0, r.pos - a.window + 1);
@@ -109,11 +110,15 @@ __device__ __forceinline__ RowUnits row_units(const AttendArgs& a, int row, int 
   return r;
 }
 
+// An item's length on the line: its units, and a fixed part that stands for
+// what every item costs beside them (fragments of q, the warps' meeting).
+__device__ __forceinline__ int line_units(const RowUnits& r) { return r.units ? r.units + kItemUnits : 0; }
+
 // The grid's cut of the line of units, and where a CTA's run starts.
 struct Run {
-  long long w0, w1, total;  // units [w0, w1) of total
-  int row;                  // row of unit w0
-  long long row_start;      // its first unit
+  long long w0, w1, total;  // [w0, w1) of the line's length
+  int row;                  // row of w0
+  long long row_start;      // where it begins
 };
 
 __device__ __forceinline__ long long run_start(long long total, int grid, int cta) {
@@ -129,7 +134,7 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
   Run run;
   long long mine = 0, x = 0, before = 0, chunk = 0;
   auto scan = [&](int r) {  // mine: units of row r; x: of the rows up to r in this chunk; chunk: of the chunk
-    mine = r < a.n_rows ? (long long)row_units(a, r, unit).units * items : 0;
+    mine = r < a.n_rows ? (long long)line_units(row_units(a, a.seqs[r], a.pos[r], unit)) * items : 0;
     x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -178,28 +183,40 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
 struct Walk {
   long long w, row_start;
   int row, item, u0, n;  // units [u0, u0 + n) of the row's item
+  int next_seq, next_pos;
   RowUnits ru;
-  bool loaded = false;
-  __device__ __forceinline__ void start(const Run& r) {
+  __device__ __forceinline__ void load_row(const AttendArgs& a) {  // of the row behind this one
+    next_seq = row + 1 < a.n_rows ? a.seqs[row + 1] : -1;
+    next_pos = row + 1 < a.n_rows ? a.pos[row + 1] : -1;
+  }
+  __device__ __forceinline__ void start(const AttendArgs& a, const Run& r, int unit) {
     w = r.w0;
     row = r.row;
     row_start = r.row_start;
-    n = 0;
+    if (w >= r.w1) return;
+    ru = row_units(a, a.seqs[row], a.pos[row], unit);
+    load_row(a);
   }
   __device__ __forceinline__ bool next(const AttendArgs& a, const Run& r, int unit, int items) {
-    w += n;
-    if (w >= r.w1) return false;
-    if (!loaded) ru = row_units(a, row, unit);
-    loaded = true;
-    while (w >= row_start + (long long)ru.units * items) {
-      row_start += (long long)ru.units * items;
-      ru = row_units(a, ++row, unit);
+    while (w < r.w1) {
+      const int len = line_units(ru);
+      if (w >= row_start + (long long)len * items) {
+        row_start += (long long)len * items;
+        ru = row_units(a, next_seq, next_pos, unit);
+        ++row;
+        load_row(a);
+        continue;
+      }
+      item = (int)((w - row_start) / len);
+      const int at = (int)(w - row_start - (long long)item * len), to = (int)min((long long)len, at + (r.w1 - w));
+      u0 = max(0, at - kItemUnits);
+      n = max(0, to - kItemUnits) - u0;
+      w += to - at;
+      if (n > 0) return true;
     }
-    item = (int)((w - row_start) / ru.units);
-    u0 = (int)(w - row_start - (long long)item * ru.units);
-    n = (int)min((long long)(ru.units - u0), r.w1 - w);
-    return true;
+    return false;
   }
+  __device__ __forceinline__ long long item_end() const { return row_start + (long long)(item + 1) * line_units(ru); }
   __device__ __forceinline__ int position(int j, int unit) const {  // first of unit u0 + j
     const int u = u0 + j;
     return (u < ru.sink_units ? u : ru.first_unit + u - ru.sink_units) * unit;
@@ -294,7 +311,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   constexpr int NW = S::kWarps, MT = S::kTiles, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
   extern __shared__ __align__(1024) uint8_t smraw[];
   __shared__ long long red[NW + 3];
-  __shared__ float q_unscale[kHeadBlock];
+  __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock];
   __shared__ float stat[NW][kHeadBlock][2];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ unsigned boxes[NS];  // the 16-position boxes of a stage that were loaded
@@ -314,7 +331,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   const Run run = find_run<S::kThreads>(a, S::kUnit, items, blockIdx.x, gridDim.x, red);
   __syncthreads();  // the barriers are set up (find_run may return before its last one)
   Walk k;
-  k.start(run);
+  k.start(a, run, S::kUnit);
   int stage = 0;
   uint32_t phase = 0;
   auto step = [&]() {
@@ -401,44 +418,72 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
     if (lane == 0) mbar_arrive(empty + stage);
     step();
   };
-  bool first = true;
-  int4 pending = make_int4(-1, 0, 0, 0);  // the item that goes on in the next CTA
-  while (k.next(a, run, S::kUnit, items)) {
+  // q of an item's heads, as the B fragments hold it (k = dims, n = heads): the
+  // values of this thread's fragment registers, read before the item begins
+  constexpr int QL = (KS + NW - 1) / NW;
+  float qv[QL][4];
+  auto load_q = [&]() {
     const int kvh = k.item / a.blocks, h0 = (k.item - kvh * a.blocks) * kHeadBlock, nh = min(kHeadBlock, a.group - h0);
     const float* q = a.q + k.row * a.q_stride + (long long)(kvh * a.group + h0) * hs;
-
-    // ---- q of the block's heads as B fragments: k = dims, n = heads
-    if (HALF) {  // a power of two per head brings its largest element to 2^13..2^14
-      for (int h = warp; h < kHeadBlock; h += NW) {
-        float m = 0.f;
-        if (h < nh)
-          for (int d = lane; d < hs; d += 32) m = fmaxf(m, fabsf(q[(long long)h * hs + d]));
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 7) | (a.q_stride & 1)) == 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        int e = 0;
-        if (m > 0.f && m < INFINITY) frexpf(m, &e);
-        if (lane == 0) q_unscale[h] = ldexpf(1.f, max(-100, min(100, e - 14)));
-      }
-      bar_compute<NW * 32>();
-    }
-    for (int i = tid; i < ks * 32; i += NW * 32) {
-      const int kk = i >> 5, h = (i & 31) >> 2, d = kk * 16 + 2 * (i & 3);
-      float x[4] = {0.f, 0.f, 0.f, 0.f};
-      if (h < nh) {
-        const float f = HALF ? 1.f / q_unscale[h] : 1.f;
+    for (int i = 0; i < QL; ++i) {
+      const int kk = warp + NW * i, h = lane >> 2, d = kk * 16 + 2 * (lane & 3);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int dd = d + (j & 1) + (j >> 1) * 8;
-          x[j] = dd < hs ? q[(long long)h * hs + dd] * f : 0.f;
+      for (int j = 0; j < 2; ++j) {
+        const float* at = q + (long long)h * hs + d + 8 * j;
+        float2 v = make_float2(0.f, 0.f);
+        if (h < nh && d + 8 * j < hs) {
+          if (vec) v = *reinterpret_cast<const float2*>(at);
+          else v = make_float2(at[0], at[1]);
         }
+        qv[i][2 * j] = v.x;
+        qv[i][2 * j + 1] = v.y;
       }
+    }
+  };
+  bool first = true, more = k.next(a, run, S::kUnit, items);
+  constexpr bool kAhead = QL <= 8;  // room in registers to read q during the meeting before
+  if (kAhead && more) load_q();
+  int4 pending = make_int4(-1, 0, 0, 0);  // the item that goes on in the next CTA
+  while (more) {
+    const int row = k.row, item = k.item, n = k.n;
+    const int kvh = item / a.blocks, h0 = (item - kvh * a.blocks) * kHeadBlock, nh = min(kHeadBlock, a.group - h0);
+    if (!kAhead) load_q();
+    if (HALF) {  // a power of two per head brings its largest element to 2^13..2^14
+      float m = 0.f;
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        uint2 b;
-        b.x = take_part<HALF>(x[0], x[1]);
-        b.y = take_part<HALF>(x[2], x[3]);
-        qf[(p * KS + kk) * 32 + (i & 31)] = b;
-      }
+      for (int i = 0; i < QL; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(qv[i][j]));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      if ((lane & 3) == 0) q_max[warp][lane >> 2] = m;
+      bar_compute<NW * 32>();
+      m = q_max[0][lane >> 2];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) m = fmaxf(m, q_max[i][lane >> 2]);
+      int e = 0;
+      if (m > 0.f && m < INFINITY) frexpf(m, &e);
+      e = max(-100, min(100, e - 14));
+      if (warp == 0 && (lane & 3) == 0) q_unscale[lane >> 2] = ldexpf(1.f, e);
+      const float f = ldexpf(1.f, -e);
+#pragma unroll
+      for (int i = 0; i < QL; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qv[i][j] *= f;
+    }
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+      const int kk = warp + NW * i;
+      if (kk < ks)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          uint2 b;
+          b.x = take_part<HALF>(qv[i][0], qv[i][1]);
+          b.y = take_part<HALF>(qv[i][2], qv[i][3]);
+          qf[(p * KS + kk) * 32 + lane] = b;
+        }
     }
     bar_compute<NW * 32>();
     float sc[2];  // score factors of this thread's two heads
@@ -450,7 +495,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 #pragma unroll
     for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int j = 0; j < k.n; ++j) {
+    for (int j = 0; j < n; ++j) {
       const int t0 = k.position(j, S::kUnit) + warp * MT * kTile;  // the warp's first position
       arrived();
       const unsigned mine = (boxes[stage] >> (warp * MT)) & ((1u << MT) - 1u);
@@ -621,7 +666,17 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
       release();
     }
 
-    // ---- the warps meet: common maximum, sums, O (added in the warps' order)
+    const bool whole = k.u0 == 0 && n == k.ru.units;
+    if (!whole && k.u0 == 0) {  // goes on in other CTAs, up to the one of the item's last unit
+      const int used = (int)min((long long)gridDim.x, run.total);
+      const long long end = k.item_end();
+      int last = blockIdx.x + 1;
+      while (run_start(run.total, used, last + 1) < end) ++last;
+      pending = make_int4(row, item, first ? 0 : 1, last);
+    }
+    // ---- the warps meet: common maximum, sums, O
+    more = k.next(a, run, S::kUnit, items);
+    if (kAhead && more) load_q();  // on its way meanwhile
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -640,47 +695,45 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
       for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][2 * (lane & 3) + h][0]);
       f[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - M);
     }
+    // few heads leave room for several warps' sums side by side; otherwise they
+    // add up in the warps' order
+    const int side = nh <= kHeadBlock / NW ? NW : nh <= kHeadBlock / 2 ? 2 : 1, width = kHeadBlock / side;
 #pragma unroll 1
-    for (int w = 0; w < NW; ++w) {
-      if (w == warp) {
+    for (int w = 0; w < NW; w += side) {
+      if (w == warp / side * side) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+          const int head = 2 * (lane & 3) + h;
+          if (head < nh) {
+            float* at = meet + ((warp - w) * width + head) * S::kPitch + (lane >> 2);
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            float* at = meet + (2 * (lane & 3) + h) * S::kPitch + i * 16 + (lane >> 2);
-            at[0] = (w ? at[0] : 0.f) + o[i][h] * f[h];
-            at[8] = (w ? at[8] : 0.f) + o[i][2 + h] * f[h];
+            for (int i = 0; i < KS; ++i) {
+              at[i * 16] = (w ? at[i * 16] : 0.f) + o[i][h] * f[h];
+              at[i * 16 + 8] = (w ? at[i * 16 + 8] : 0.f) + o[i][2 + h] * f[h];
+            }
           }
+        }
       }
       bar_compute<NW * 32>();
     }
-    const bool whole = k.u0 == 0 && k.n == k.ru.units;
-    for (int e = tid; e < nh * hs; e += NW * 32) {
-      const int h = e / hs, d = e - h * hs;
+    for (int h = warp; h < nh; h += NW) {
       float M = -INFINITY, L = 0.f;
 #pragma unroll
       for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][h][0]);
 #pragma unroll
       for (int i = 0; i < NW; ++i) L += stat[i][h][0] == -INFINITY ? 0.f : exp2_approx(stat[i][h][0] - M) * stat[i][h][1];
-      const float acc = meet[h * S::kPitch + d];
-      if (whole) {
-        a.out[k.row * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d] = L > 0.f ? acc / L : 0.f;
-      } else {
-        float* ws = a.ws + ((long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock + h) * (hs + 2);
-        if (d == 0) {
-          ws[0] = M;
-          ws[1] = L;
-        }
-        ws[2 + d] = acc;
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+      float* ws = a.ws + ((long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock + h) * (hs + 2);
+      float* out = whole ? a.out + row * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs : ws + 2;
+      if (!whole && lane == 0) {
+        ws[0] = M;
+        ws[1] = L;
       }
-    }
-    if (!whole && k.u0 == 0) pending = make_int4(k.row, k.item, first ? 0 : 1, 0);
-    if (pending.x >= 0 && pending.w == 0) {  // the CTA of the item's last unit
-      const int used = (int)min((long long)gridDim.x, run.total);
-      const long long end = k.w + k.ru.units;
-      int last = blockIdx.x + 1;
-      while (run_start(run.total, used, last + 1) < end) ++last;
-      pending.w = last;
+      for (int d = lane; d < hs; d += 32) {
+        float acc = meet[h * S::kPitch + d];
+        for (int i = 1; i < side; ++i) acc += meet[(i * width + h) * S::kPitch + d];
+        out[d] = whole ? acc * inv : acc;
+      }
     }
     bar_compute<NW * 32>();  // the meeting place and the statistics are free again
     first = false;
