@@ -251,11 +251,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 template <bool HALF>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -309,6 +309,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   using S = AttendShape<TYPE, HSP>;
   constexpr bool HALF = TYPE == F16;
   constexpr int NW = S::kWarps, MT = S::kTiles, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
+  constexpr int KG = 4;  // mma steps whose operands are read together: a 128-byte block of a 16-bit head
   extern __shared__ __align__(1024) uint8_t smraw[];
   __shared__ long long red[NW + 3];
   __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock];
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 #pragma unroll
     for (int i = 0; i < QL; ++i) {
       const int kk = warp + NW * i;
-      if (kk < ks)
+      if (kk < KS)
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           uint2 b;
@@ -508,26 +509,35 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
       uint32_t pf[MT][NP][2];
       bool partial = false;
       {
-        float s[MT][NP][4];
+        // sums by part and by even and odd step: enough independent chains to
+        // cover an mma's latency
+        float s[MT][2][NP][4];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) s[t][p][0] = s[t][p][1] = s[t][p][2] = s[t][p][3] = 0.f;
+          for (int p = 0; p < 2 * NP; ++p) s[t][p / NP][p % NP][0] = s[t][p / NP][p % NP][1] = s[t][p / NP][p % NP][2] = s[t][p / NP][p % NP][3] = 0.f;
         const uint32_t kt = ring + stage * S::kStage;
         const uint8_t* kg = smraw + stage * S::kStage;
         if (TYPE != F32) {
-#pragma unroll 4
-          for (int kk = 0; kk < ks; ++kk) {
-            uint2 b[NP];
+          // steps behind the head's end multiply what the map filled with zeros
+#pragma unroll 2
+          for (int k0 = 0; k0 < ks; k0 += KG) {
+            uint2 b[KG][NP];
+            uint32_t ka[KG][MT][4];
 #pragma unroll
-            for (int p = 0; p < NP; ++p) b[p] = qf[(p * KS + kk) * 32 + lane];
+            for (int g = 0; g < KG; ++g) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              uint32_t ka[4];
-              ldsm4(ka, kt + chunk_at<BLK>((warp * MT + t) * kTile + (lane & 15), 2 * kk + (lane >> 4)));
+              for (int p = 0; p < NP; ++p) b[g][p] = qf[(p * KS + k0 + g) * 32 + lane];
 #pragma unroll
-              for (int p = 0; p < NP; ++p) mma16816<HALF>(s[t][p], ka, b[p].x, b[p].y);
+              for (int t = 0; t < MT; ++t)
+                ldsm4(ka[g][t], kt + chunk_at<BLK>((warp * MT + t) * kTile + (lane & 15), 2 * (k0 + g) + (lane >> 4)));
             }
+#pragma unroll
+            for (int g = 0; g < KG; ++g)
+#pragma unroll
+              for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][g & 1][p], ka[g][t], b[g][p].x, b[g][p].y);
           }
         } else {
 #pragma unroll 2
@@ -552,7 +562,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
               for (int p = 0; p < NP; ++p) {  // products of parts i + p <= 2
                 const uint2 b = qf[(p * KS + kk) * 32 + lane];
 #pragma unroll
-                for (int i = 0; i < 3 - p; ++i) mma16816<false>(s[t][i], ka[i], b.x, b.y);
+                for (int i = 0; i < 3 - p; ++i) mma16816<false>(s[t][p & 1][i], ka[i], b.x, b.y);
               }
             }
           }
@@ -567,9 +577,9 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
           partial |= !whole;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = s[t][NP - 1][i];
+            float v = s[t][0][NP - 1][i] + s[t][1][NP - 1][i];
 #pragma unroll
-            for (int p = NP - 2; p >= 0; --p) v += s[t][p][i];
+            for (int p = NP - 2; p >= 0; --p) v += s[t][0][p][i] + s[t][1][p][i];
             const bool vis = whole || (have && k.seen(tt + (lane >> 2) + (i >> 1) * 8, a.sinks));
             x[t][i] = vis ? v * sc[i & 1] : -INFINITY;
           }
@@ -629,18 +639,30 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
+        if (TYPE != F32) {
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          if (i < ks) {
+          for (int i = 0; i < KS; i += KG) {
+            if (i < ks) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              if (TYPE != F32) {
-                uint32_t va[4];
+              for (int t = 0; t < MT; ++t) {
+                uint32_t va[KG][4];
                 const int r = (warp * MT + t) * kTile + (lane & 7) + (lane >> 4) * 8;
-                ldsm4_t(va, vt + chunk_at<BLK>(r, 2 * i + ((lane >> 3) & 1)));
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p) mma16816<HALF>(o[i], va, pf[t][p][0], pf[t][p][1]);
-              } else {
+                for (int g = 0; g < KG; ++g)
+                  ldsm4_t(va[g], vt + chunk_at<BLK>(r, 2 * (i + g) + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                  for (int g = 0; g < KG; ++g) mma16816<HALF>(o[i + g], va[g], pf[t][p][0], pf[t][p][1]);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            if (i < ks) {
+#pragma unroll
+              for (int t = 0; t < MT; ++t) {
                 // V[pos 2 (lane % 4) + {0, 1} (+ 8)][dim lane / 4 (+ 8)]: registers (dim), (dim + 8), then pos + 8
                 float x[8];
 #pragma unroll
