@@ -9,10 +9,12 @@
 // The turns are reduced to [-1/2, 1/2] in 64 bits and only then rounded, so the
 // angle is right to 1e-7 at every position.
 //
-// Bound by HBM: every input and output element moves once.  A warp owns one
-// head vector at a time: its elements stay in registers as groups of four (two
-// pairs), the squares are summed by shuffles, and the cosines and sines of a
-// row are computed once per warp and used for all heads the warp takes.
+// Bound by HBM: every input and output element moves once.  A warp owns a head
+// vector: its elements stay in registers as groups of four (two pairs), the
+// squares are summed by shuffles. The cosines and sines of a row are computed
+// once per CTA (64-bit products and conversions cost as much as the row's
+// memory traffic when every warp repeats them) while the heads' elements are on
+// their way.
 #include "g4_common.cuh"
 #include "g4_kv.h"
 
@@ -30,7 +32,7 @@ struct g4_rope {
 
 namespace g4 {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256;
 
 struct AppendArgs {
   const float *q, *k, *v;
@@ -49,7 +51,7 @@ struct AppendArgs {
   const int32_t *table, *refs;
   unsigned* flags;
   int n_seqs, max_pages, max_positions, page_shift, n_pages;
-  int heads_per_warp, warps_per_row;
+  int heads_per_cta, ctas_per_row;
 };
 
 template <int TYPE>
@@ -62,110 +64,156 @@ __device__ __forceinline__ void store2(uint8_t* base, long long at, float x, flo
     reinterpret_cast<__nv_bfloat162*>(base)[at / 2] = __floats2bfloat162_rn(x, y);
   }
 }
-
-// NQ groups of four elements per lane: head sizes up to 128 * NQ.
-template <int TYPE, int NQ>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
-  const long long row = w / a.warps_per_row;
-  if (row >= a.n_rows) return;
-  const int heads = a.n_q + 2 * a.n_kv;
-  const int h0 = (int)(w - row * a.warps_per_row) * a.heads_per_warp, h1 = min(h0 + a.heads_per_warp, heads);
-  const int seq = a.seqs ? a.seqs[row] : 0, pos = a.pos[row];
-  if (seq < 0) return;  // a padding row
-  if (pos < 0 || (a.k && (seq >= a.n_seqs || pos >= a.max_positions))) {
-    if (lane == 0 && a.flags) atomicOr(a.flags, KV_BAD_ROW);
-    return;
+template <int TYPE>
+__device__ __forceinline__ void store4(uint8_t* base, long long at, float4 v) {
+  if (TYPE == F32) {
+    reinterpret_cast<float4*>(base)[at / 4] = v;
+  } else {
+    uint2 u;
+    if (TYPE == F16) {
+      const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+      u = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+      u = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+    reinterpret_cast<uint2*>(base)[at / 4] = u;
   }
-  const int half = a.rot / 2, quads = a.hs / 4, rq = a.rot / 4;
-  // element offsets of each of the lane's groups: pairs (lo, hi), (lo + 1, hi + 1) or consecutive elements
-  int lo[NQ], hi[NQ];
-  float cs[NQ][2], sn[NQ][2];
+}
+
+// NQ groups of four elements per lane (head sizes up to 128 * NQ), HB heads of
+// a warp in flight together. A CTA takes heads_per_cta heads of one row; its
+// warps share the row's cosines and sines.
+template <int TYPE, int NQ, int HB>
+__global__ void __launch_bounds__(kAppendThreads, NQ * HB <= 6 ? 4 : 2)
+    kv_append_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ float4 turn[kKvMaxHeadSize / 4];  // cosine and sine of a group's two pairs
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int NW = kAppendThreads / 32;
+  const long long row = blockIdx.x / a.ctas_per_row;
+  const int heads = a.n_q + 2 * a.n_kv, quads = a.hs / 4, rq = a.rot / 4, half = a.rot / 2;
+  const int c0 = (int)(blockIdx.x - row * a.ctas_per_row) * a.heads_per_cta;
+  const int h0 = c0 + warp, h1 = min(c0 + a.heads_per_cta, heads);  // every NW-th head
+  // a group is two pairs: elements (2m, 2m + 1) with (2m, 2m + 1) + rot / 2, or four consecutive ones
+  bool split[NQ];
+  int lo[NQ];
 #pragma unroll
   for (int u = 0; u < NQ; ++u) {
     const int m = lane + 32 * u;
-    const bool split = m < rq && !a.interleaved;
-    lo[u] = split ? 2 * m : 4 * m;
-    hi[u] = split ? 2 * m + half : 4 * m + 2;
+    split[u] = m < rq && !a.interleaved;
+    lo[u] = split[u] ? 2 * m : 4 * m;
+  }
+  auto source = [&](int h) {
+    return h < a.n_q             ? a.q + row * a.q_stride + (long long)h * a.hs
+           : h < a.n_q + a.n_kv  ? a.k + row * a.k_stride + (long long)(h - a.n_q) * a.hs
+                                 : a.v + row * a.v_stride + (long long)(h - a.n_q - a.n_kv) * a.hs;
+  };
+  auto load = [&](int h, float4 (&x)[NQ]) {
+    const float* p = source(h);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      cs[u][j] = 1.f;
-      sn[u][j] = 0.f;
-      if (m < rq) {
-        const double t = (double)pos * a.turns[2 * m + j];
-        float s, c;
-        sincospif(2.f * (float)(t - rint(t)), &s, &c);
-        cs[u][j] = c * a.factor;
-        sn[u][j] = s * a.factor;
+    for (int u = 0; u < NQ; ++u) {
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (lane + 32 * u >= quads) continue;
+      if (split[u]) {
+        const float2 f = __ldcs(reinterpret_cast<const float2*>(p + lo[u]));
+        const float2 g = __ldcs(reinterpret_cast<const float2*>(p + lo[u] + half));
+        x[u] = make_float4(f.x, f.y, g.x, g.y);
+      } else {
+        x[u] = __ldcs(reinterpret_cast<const float4*>(p + lo[u]));
       }
     }
+  };
+  // the first heads' elements are on their way before the row's position is known
+  float4 x[HB][NQ];
+#pragma unroll
+  for (int i = 0; i < HB; ++i)
+    if (h0 + i * NW < h1) load(h0 + i * NW, x[i]);
+  const int seq = a.seqs ? a.seqs[row] : 0, pos = a.pos[row];
+  if (seq < 0) return;  // a padding row
+  if (pos < 0 || (a.k && (seq >= a.n_seqs || pos >= a.max_positions))) {
+    if (threadIdx.x == 0 && a.flags) atomicOr(a.flags, KV_BAD_ROW);
+    return;
   }
   // the row's page: a position without one, or in a page that sequences share, is not stored
-  long long slot = -1;
-  if (a.k && h1 > a.n_q) {
-    const int page = a.table[(long long)seq * a.max_pages + (pos >> a.page_shift)];
-    const bool ok = (unsigned)page < (unsigned)a.n_pages && a.refs[page] <= 1;
-    if (ok) slot = (((long long)page * a.n_kv) << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-    else if (lane == 0) atomicOr(a.flags, KV_NOT_STORED);
+  const bool stores = a.k && h1 > a.n_q;
+  const int page = stores ? a.table[(long long)seq * a.max_pages + (pos >> a.page_shift)] : -1;
+  for (int m = threadIdx.x; m < 2 * rq; m += kAppendThreads) {
+    const double t = (double)pos * a.turns[m];
+    float s, c;
+    sincospif(2.f * (float)(t - rint(t)), &s, &c);
+    reinterpret_cast<float2*>(turn)[m] = make_float2(c * a.factor, s * a.factor);
   }
-  for (int h = h0; h < h1; ++h) {
-    const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
-    const int hh = is_q ? h : is_k ? h - a.n_q : h - a.n_q - a.n_kv;
-    if (!is_q && slot < 0) break;
-    const float* x = (is_q ? a.q + row * a.q_stride : is_k ? a.k + row * a.k_stride : a.v + row * a.v_stride) +
-                     (long long)hh * a.hs;
-    float2 p[NQ], r[NQ];
-    float ss = 0.f;
+  const bool known = (unsigned)page < (unsigned)a.n_pages;
+  const int refs = known ? a.refs[page] : 2;
+  __syncthreads();
+  long long slot = -1;
+  if (refs <= 1) slot = (((long long)page * a.n_kv) << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+  else if (stores && threadIdx.x == 0) atomicOr(a.flags, KV_NOT_STORED);
+  float4 cs[NQ];
 #pragma unroll
-    for (int u = 0; u < NQ; ++u) {
-      p[u] = r[u] = make_float2(0.f, 0.f);
-      if (lane + 32 * u < quads) {
-        p[u] = __ldcs(reinterpret_cast<const float2*>(x + lo[u]));
-        r[u] = __ldcs(reinterpret_cast<const float2*>(x + hi[u]));
-      }
-      ss += p[u].x * p[u].x + p[u].y * p[u].y + r[u].x * r[u].x + r[u].y * r[u].y;
-    }
-    const float* nw = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
-    if (nw || (!is_q && !is_k && a.norm_v)) {
-      const float s = rms_scale(warp_sum(ss), a.hs, a.eps);
+  for (int u = 0; u < NQ; ++u) cs[u] = lane + 32 * u < rq ? turn[lane + 32 * u] : make_float4(1.f, 0.f, 1.f, 0.f);
+  for (int hb = h0; hb < h1; hb += HB * NW) {
+    if (hb > h0) {
 #pragma unroll
-      for (int u = 0; u < NQ; ++u)
-        if (lane + 32 * u < quads) {
-          const float2 one = make_float2(1.f, 1.f);
-          const float2 wp = nw ? __ldg(reinterpret_cast<const float2*>(nw + lo[u])) : one;
-          const float2 wr = nw ? __ldg(reinterpret_cast<const float2*>(nw + hi[u])) : one;
-          p[u].x *= wp.x * s;
-          p[u].y *= wp.y * s;
-          r[u].x *= wr.x * s;
-          r[u].y *= wr.y * s;
-        }
+      for (int i = 0; i < HB; ++i)
+        if (hb + i * NW < h1) load(hb + i * NW, x[i]);
     }
 #pragma unroll
-    for (int u = 0; u < NQ; ++u) {
-      if (lane + 32 * u >= quads) continue;
-      if (is_q || is_k) {
-        // split layout: pairs (p.x, r.x), (p.y, r.y); interleaved: (p.x, p.y), (r.x, r.y)
-        float a0 = p[u].x, b0 = r[u].x, a1 = p[u].y, b1 = r[u].y;
-        const bool inter = a.interleaved;
-        if (inter) {
-          b0 = p[u].y;
-          a1 = r[u].x;
+    for (int i = 0; i < HB; ++i) {
+      const int h = hb + i * NW;
+      const bool is_q = h < a.n_q, is_k = !is_q && h < a.n_q + a.n_kv;
+      if (h >= h1 || (!is_q && slot < 0)) break;
+      const int hh = is_q ? h : is_k ? h - a.n_q : h - a.n_q - a.n_kv;
+      const float* nw = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+      if (nw || (!is_q && !is_k && a.norm_v)) {
+        float ss = 0.f;
+#pragma unroll
+        for (int u = 0; u < NQ; ++u)
+          ss += x[i][u].x * x[i][u].x + x[i][u].y * x[i][u].y + x[i][u].z * x[i][u].z + x[i][u].w * x[i][u].w;
+        const float s = rms_scale(warp_sum(ss), a.hs, a.eps);
+#pragma unroll
+        for (int u = 0; u < NQ; ++u) {
+          if (lane + 32 * u >= quads) continue;
+          float2 f = make_float2(1.f, 1.f), g = f;
+          if (nw) {
+            f = __ldg(reinterpret_cast<const float2*>(nw + lo[u]));
+            g = __ldg(reinterpret_cast<const float2*>(nw + lo[u] + (split[u] ? half : 2)));
+          }
+          x[i][u].x *= f.x * s;
+          x[i][u].y *= f.y * s;
+          x[i][u].z *= g.x * s;
+          x[i][u].w *= g.y * s;
         }
-        const float y0 = a0 * cs[u][0] - b0 * sn[u][0], z0 = a0 * sn[u][0] + b0 * cs[u][0];
-        const float y1 = a1 * cs[u][1] - b1 * sn[u][1], z1 = a1 * sn[u][1] + b1 * cs[u][1];
-        p[u] = inter ? make_float2(y0, z0) : make_float2(y0, y1);
-        r[u] = inter ? make_float2(y1, z1) : make_float2(z0, z1);
       }
-      if (is_q) {
-        float* o = a.q_out + row * a.out_stride + (long long)hh * a.hs;
-        *reinterpret_cast<float2*>(o + lo[u]) = p[u];
-        *reinterpret_cast<float2*>(o + hi[u]) = r[u];
-      } else {
-        const long long at = (slot + ((long long)hh << a.page_shift)) * a.hs;
-        uint8_t* pool = is_k ? a.kp : a.vp;
-        store2<TYPE>(pool, at + lo[u], p[u].x, p[u].y);
-        store2<TYPE>(pool, at + hi[u], r[u].x, r[u].y);
+#pragma unroll
+      for (int u = 0; u < NQ; ++u) {
+        if (lane + 32 * u >= quads) continue;
+        float4 v = x[i][u];
+        if (is_q || is_k) {
+          // pairs (x, z), (y, w) of a split group, (x, y), (z, w) otherwise
+          const float b0 = split[u] ? v.z : v.y, a1 = split[u] ? v.y : v.z;
+          const float y0 = v.x * cs[u].x - b0 * cs[u].y, z0 = v.x * cs[u].y + b0 * cs[u].x;
+          const float y1 = a1 * cs[u].z - v.w * cs[u].w, z1 = a1 * cs[u].w + v.w * cs[u].z;
+          v = split[u] ? make_float4(y0, y1, z0, z1) : make_float4(y0, z0, y1, z1);
+        }
+        if (is_q) {
+          float* o = a.q_out + row * a.out_stride + (long long)hh * a.hs;
+          if (split[u]) {
+            *reinterpret_cast<float2*>(o + lo[u]) = make_float2(v.x, v.y);
+            *reinterpret_cast<float2*>(o + lo[u] + half) = make_float2(v.z, v.w);
+          } else {
+            *reinterpret_cast<float4*>(o + lo[u]) = v;
+          }
+        } else {
+          const long long at = (slot + ((long long)hh << a.page_shift)) * a.hs + lo[u];
+          uint8_t* pool = is_k ? a.kp : a.vp;
+          if (split[u]) {
+            store2<TYPE>(pool, at, v.x, v.y);
+            store2<TYPE>(pool, at + half, v.z, v.w);
+          } else {
+            store4<TYPE>(pool, at, v);
+          }
+        }
       }
     }
   }
@@ -173,27 +221,29 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 
 using AppendFn = void (*)(const AppendArgs);
 template <int TYPE>
-static AppendFn append_fn_t(int hs) {
-  return hs <= 128 ? kv_append_kernel<TYPE, 1> : hs <= 256 ? kv_append_kernel<TYPE, 2> : kv_append_kernel<TYPE, 4>;
+static AppendFn append_fn_t(int hs, bool many) {
+  if (many) return hs <= 128 ? kv_append_kernel<TYPE, 1, 6> : hs <= 256 ? kv_append_kernel<TYPE, 2, 3> : kv_append_kernel<TYPE, 4, 2>;
+  return hs <= 128 ? kv_append_kernel<TYPE, 1, 1> : hs <= 256 ? kv_append_kernel<TYPE, 2, 1> : kv_append_kernel<TYPE, 4, 1>;
 }
-static AppendFn append_fn(int type, int hs) {
-  return type == F32 ? append_fn_t<F32>(hs) : type == F16 ? append_fn_t<F16>(hs) : append_fn_t<BF16>(hs);
+static AppendFn append_fn(int type, int hs, bool many) {
+  return type == F32   ? append_fn_t<F32>(hs, many)
+         : type == F16 ? append_fn_t<F16>(hs, many)
+                       : append_fn_t<BF16>(hs, many);
 }
 
 static cudaError_t launch_append(const DeviceInfo& dev, int type, AppendArgs a, cudaStream_t st) {
   const int heads = a.n_q + (a.k ? 2 * a.n_kv : 0);
   if (!a.k) a.n_kv = 0;
   // Heads per warp: one while the rows do not fill the GPU (a decode step is
-  // latency: every head vector its own warp), eight once every SM has 64 warps
-  // of that many, which shares a row's cosines and sines.
-  const long long all = (long long)a.n_rows * heads;
-  const long long full = (long long)dev.sms * 64;
-  a.heads_per_warp = all >= 8 * full ? 8 : all >= 4 * full ? 4 : all >= 2 * full ? 2 : 1;
-  a.warps_per_row = (heads + a.heads_per_warp - 1) / a.heads_per_warp;
-  const long long warps = (long long)a.n_rows * a.warps_per_row;
-  const long long grid = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+  // latency: every head vector its own warp); a whole row per CTA, up to four
+  // heads of a warp in flight, once that leaves every SM 32 warps.
+  constexpr int kWarps = kAppendThreads / 32;
+  const bool many = (long long)a.n_rows * kWarps >= (long long)dev.sms * 32;
+  a.heads_per_cta = many ? heads : kWarps;
+  a.ctas_per_row = (heads + a.heads_per_cta - 1) / a.heads_per_cta;
+  const long long grid = (long long)a.n_rows * a.ctas_per_row;
   if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
-  append_fn(type, a.hs)<<<(unsigned)grid, kAppendThreads, 0, st>>>(a);
+  append_fn(type, a.hs, many && heads > kWarps)<<<(unsigned)grid, kAppendThreads, 0, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -202,7 +252,8 @@ int rope_prepare() {
   cudaError_t e = cudaSuccess;
   for (int type : {F32, F16, BF16})
     for (int hs : {128, 256, 512})
-      if (!e) e = cudaFuncGetAttributes(&fa, append_fn(type, hs));
+      for (bool many : {false, true})
+        if (!e) e = cudaFuncGetAttributes(&fa, append_fn(type, hs, many));
   return e;
 }
 
