@@ -85,7 +85,7 @@ __device__ __forceinline__ void store4(uint8_t* base, long long at, float4 v) {
 // a warp in flight together. A CTA takes heads_per_cta heads of one row; its
 // warps share the row's cosines and sines.
 template <int TYPE, int NQ, int HB>
-__global__ void __launch_bounds__(kAppendThreads, NQ * HB <= 6 ? 4 : 2)
+__global__ void __launch_bounds__(kAppendThreads, NQ == 1 ? 7 : NQ == 2 ? 6 : 4)
     kv_append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ float4 turn[kKvMaxHeadSize / 4];  // cosine and sine of a group's two pairs
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -115,11 +115,11 @@ __global__ void __launch_bounds__(kAppendThreads, NQ * HB <= 6 ? 4 : 2)
       x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (lane + 32 * u >= quads) continue;
       if (split[u]) {
-        const float2 f = __ldcs(reinterpret_cast<const float2*>(p + lo[u]));
-        const float2 g = __ldcs(reinterpret_cast<const float2*>(p + lo[u] + half));
+        const float2 f = __ldg(reinterpret_cast<const float2*>(p + lo[u]));
+        const float2 g = __ldg(reinterpret_cast<const float2*>(p + lo[u] + half));
         x[u] = make_float4(f.x, f.y, g.x, g.y);
       } else {
-        x[u] = __ldcs(reinterpret_cast<const float4*>(p + lo[u]));
+        x[u] = __ldg(reinterpret_cast<const float4*>(p + lo[u]));
       }
     }
   };
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kAppendThreads, NQ * HB <= 6 ? 4 : 2)
 #pragma unroll
         for (int u = 0; u < NQ; ++u)
           ss += x[i][u].x * x[i][u].x + x[i][u].y * x[i][u].y + x[i][u].z * x[i][u].z + x[i][u].w * x[i][u].w;
-        const float s = rms_scale(warp_sum(ss), a.hs, a.eps);
+        const float s = rsqrtf(warp_sum(ss) / a.hs + a.eps);
 #pragma unroll
         for (int u = 0; u < NQ; ++u) {
           if (lane + 32 * u >= quads) continue;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(kAppendThreads, NQ * HB <= 6 ? 4 : 2)
 using AppendFn = void (*)(const AppendArgs);
 template <int TYPE>
 static AppendFn append_fn_t(int hs, bool many) {
-  if (many) return hs <= 128 ? kv_append_kernel<TYPE, 1, 6> : hs <= 256 ? kv_append_kernel<TYPE, 2, 3> : kv_append_kernel<TYPE, 4, 2>;
+  if (many) return hs <= 128 ? kv_append_kernel<TYPE, 1, 2> : hs <= 256 ? kv_append_kernel<TYPE, 2, 1> : kv_append_kernel<TYPE, 4, 1>;
   return hs <= 128 ? kv_append_kernel<TYPE, 1, 1> : hs <= 256 ? kv_append_kernel<TYPE, 2, 1> : kv_append_kernel<TYPE, 4, 1>;
 }
 static AppendFn append_fn(int type, int hs, bool many) {
