@@ -4,8 +4,9 @@
 // One pass over the logits (bound by HBM: 4 bytes a candidate).  A CTA holds
 // kChunk logits of a row in registers and takes from them the chunk's maximum
 // and sum of exponentials and its `beams` largest logits: the beams-th largest
-// of the threads' own maxima bounds them from below, so only candidates at or
-// above it (beams to 32 * beams of kChunk) are ranked, by counting.  A second
+// of the threads' own maxima bounds them from below (the warps sort theirs and
+// rank them in each other's lists), so only candidates at or above it (beams to
+// 32 * beams of kChunk) are ranked, by counting.  A second
 // launch joins a group's chunks: the log sums in 64 bits, then the best
 // continuations by the same ranking, on 64-bit scores.
 //
@@ -38,13 +39,27 @@ struct ChunkStat {
   float m, sum;
 };
 
-__global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const float* logits, long long stride, int vocab,
-                                                                  const int32_t* finished, int beams, int chunks,
-                                                                  unsigned long long* best, ChunkStat* stats) {
-  __shared__ unsigned long long top[kBeamThreads];
+// The lanes' keys in descending order (bitonic).
+__device__ __forceinline__ unsigned long long warp_sort(unsigned long long k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+      const bool keep_max = ((lane & o) == 0) == ((lane & size) == 0);
+      k = (other > k) == keep_max ? other : k;
+    }
+  return k;
+}
+
+__global__ void __launch_bounds__(kBeamThreads, 4)
+    beam_chunk_kernel(const float* logits, long long stride, int vocab, const int32_t* finished, int beams, int chunks,
+                      unsigned long long* best, ChunkStat* stats) {
+  constexpr int NW = kBeamThreads / 32, G = kBeamPer / 4;
+  __shared__ unsigned long long top[NW][kMaxBeams];
   __shared__ unsigned long long cand[kMaxBeams * kBeamPer];
   __shared__ unsigned long long bound_s;
-  __shared__ float red[kBeamThreads / 32];
+  __shared__ float red[NW];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
@@ -53,66 +68,91 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const float* l
   const float* x = logits + row * stride;
   const int t0 = c * kChunk;
   if (tid == 0) count = 0;
-  // element i of a thread: token t0 + (i / 4) * 1024 + 4 tid + i % 4
-  float v[kBeamPer];
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  // group i of a thread: tokens t0 + i * 1024 + 4 tid + {0..3}
+  float v[G][4];
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && t0 + kChunk <= vocab;
+  if (vec) {
 #pragma unroll
-  for (int i = 0; i < kBeamPer / 4; ++i) {
-    const int t = t0 + (i * kBeamThreads + tid) * 4;
-    if (vec && t + 4 <= vocab) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + t));
-      v[4 * i] = f.x;
-      v[4 * i + 1] = f.y;
-      v[4 * i + 2] = f.z;
-      v[4 * i + 3] = f.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[4 * i + j] = t + j < vocab ? x[t + j] : -INFINITY;
+    for (int i = 0; i < G; ++i) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + t0 + (i * kBeamThreads + tid) * 4));
+      v[i][0] = f.x;
+      v[i][1] = f.y;
+      v[i][2] = f.z;
+      v[i][3] = f.w;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = t0 + (i * kBeamThreads + tid) * 4 + j;
+        v[i][j] = t < vocab ? x[t] : -INFINITY;
+      }
   }
+  // the thread's largest logit (a NaN is never the larger one) and its group
   float m = -INFINITY;
   int at = 0;
 #pragma unroll
-  for (int i = 0; i < kBeamPer; ++i) {
-    if (!(v[i] == v[i])) v[i] = -INFINITY;  // a NaN is never chosen
-    if (v[i] > m) {
-      m = v[i];
+  for (int i = 0; i < G; ++i) {
+    const float g = fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3]));
+    if (g > m) {
+      m = g;
       at = i;
     }
   }
-  auto token_of = [&](int i) { return t0 + ((i >> 2) * kBeamThreads + tid) * 4 + (i & 3); };
   auto key_of = [&](float f, int token) {
     return ((unsigned long long)order_of(f) << 32) | (0xffffffffu - (uint32_t)token);
   };
-  const unsigned long long mine = key_of(m, token_of(at));
-  top[tid] = mine;
-  float M = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if (lane == 0) red[warp] = M;
+  // The bound: the beams-th largest of the threads' keys, a key being the
+  // largest logit with its group's last token, so at most that of the logit
+  // itself: beams candidates reach it, all in threads whose keys do.
+  const unsigned long long mine = key_of(m, t0 + (at * kBeamThreads + tid) * 4 + 3);
+  const unsigned long long sorted = warp_sort(mine, lane);
+  if (lane < beams) top[warp][lane] = sorted;
+  const float warp_max = value_of((uint32_t)(__shfl_sync(0xffffffffu, sorted, 0) >> 32));
+  if (lane == 0) red[warp] = warp_max;
   __syncthreads();
+  float M = red[0];
 #pragma unroll
-  for (int i = 0; i < kBeamThreads / 32; ++i) M = fmaxf(M, red[i]);
-  // the bound: the beams-th largest of the threads' maxima
-  int rank = 0;
-  for (int i = 0; i < kBeamThreads; ++i) rank += top[i] > mine;
-  if (rank == beams - 1) bound_s = mine;
+  for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
+  if (lane < beams) {
+    int rank = lane;
+    for (int w = 1; w < NW; ++w) {  // in another warp's list: how many are larger
+      const unsigned long long* list = top[(warp + w) % NW];
+      int r = 0;
+      for (int i = 0; i < beams && list[i] > sorted; ++i) ++r;
+      rank += r;
+    }
+    if (rank == beams - 1) bound_s = sorted;
+  }
   const float base = M == -INFINITY ? 0.f : M;
-  float s = 0.f;
+  float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBeamPer; ++i) s += __expf(v[i] - base);
-  s = warp_sum(s);
+  for (int i = 0; i < G; ++i) {
+    s0 += __expf(v[i][0] - base) + __expf(v[i][1] - base);
+    s1 += __expf(v[i][2] - base) + __expf(v[i][3] - base);
+  }
+  if (!(s0 + s1 == s0 + s1)) {  // NaNs count as masked
+    s0 = s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s0 += v[i][j] == v[i][j] ? __expf(v[i][j] - base) : 0.f;
+  }
+  const float sum = warp_sum(s0 + s1);
   __syncthreads();
-  if (lane == 0) red[warp] = s;
+  if (lane == 0) red[warp] = sum;
   const unsigned long long bound = bound_s;
-  const float bv = value_of((uint32_t)(bound >> 32));
-  if (mine >= bound) {  // only these threads can hold candidates
+  if (mine >= bound) {
+    const float bv = value_of((uint32_t)(bound >> 32));
 #pragma unroll
-    for (int i = 0; i < kBeamPer; ++i)
-      if (v[i] >= bv) {
-        const unsigned long long k = key_of(v[i], token_of(i));
-        if (k >= bound) cand[atomicAdd(&count, 1)] = k;
-      }
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v[i][j] >= bv) {
+          const unsigned long long k = key_of(v[i][j], t0 + (i * kBeamThreads + tid) * 4 + j);
+          if (k >= bound) cand[atomicAdd(&count, 1)] = k;
+        }
   }
   __syncthreads();
   const int n = count;
@@ -126,7 +166,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_chunk_kernel(const float* l
   if (tid == 0) {
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < kBeamThreads / 32; ++i) t += red[i];
+    for (int i = 0; i < NW; ++i) t += red[i];
     stats[(long long)row * chunks + c] = ChunkStat{M, t};
   }
 }
@@ -154,33 +194,33 @@ __global__ void __launch_bounds__(kBeamJoinThreads) beam_join_kernel(
     const int row = g0 + b;
     if (finished && finished[row]) continue;
     const ChunkStat* st = stats + (long long)row * chunks;
+    const unsigned long long* list = best + (long long)row * chunks * beams;
+    // the row's best: sorted blocks of 32 keys, the lists' heads first; a block
+    // is looked at only if it can hold one of the best so far
+    unsigned long long kept = 0;  // lane i: the i-th largest so far
+    const int total = chunks * beams;
     float M = -INFINITY;
     for (int i = lane; i < chunks; i += 32) M = fmaxf(M, st[i].m);
+    for (int i0 = 0; i0 < total; i0 += 32) {
+      // element i of this order: head i / chunks of chunk i % chunks
+      const int i = i0 + lane, head = i / chunks;
+      unsigned long long k = i < total ? list[(long long)(i - head * chunks) * beams + head] : 0;
+      const unsigned long long least = __shfl_sync(0xffffffffu, kept, beams - 1);
+      if (!__any_sync(0xffffffffu, k > least)) continue;
+      k = warp_sort(k, lane);
+      // both lists descend: the larger of element i and element 31 - i of the other are the 32 largest
+      const unsigned long long other = __shfl_sync(0xffffffffu, k, 31 - lane);
+      kept = warp_sort(other > kept ? other : kept, lane);
+    }
+    if (lane < beams) row_key[b][lane] = kept;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     double s = 0.0;
     for (int i = lane; i < chunks; i += 32)
-      if (st[i].m > -INFINITY) s += (double)st[i].sum * exp((double)st[i].m - (double)M);
+      if (st[i].m > -INFINITY) s += (double)(st[i].sum * expf(st[i].m - M));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if (lane == 0) lse[b] = M == -INFINITY ? INFINITY : (double)M + log(s);
-    // the row's best: repeatedly the largest head of the chunks' ordered lists
-    const unsigned long long* list = best + (long long)row * chunks * beams;
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < beams; ++k) {
-      unsigned long long x = 0;
-      for (int i = lane; i < chunks * beams; i += 32) {
-        const unsigned long long y = list[i];
-        if (y < last && y > x) x = y;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, o);
-        x = y > x ? y : x;
-      }
-      if (lane == 0) row_key[b][k] = x;
-      last = x;
-    }
   }
   __syncthreads();
   const int n = beams * beams;
