@@ -1,31 +1,41 @@
 // g4_beam.cu -- beam search's selection: for every group of `beams` rows, the
 // `beams` best of all continuations score_b + logit_bt - log sum_t exp(logit_bt).
 //
-// One pass over the logits (bound by HBM: 4 bytes a candidate).  A CTA holds
-// kChunk logits of a row in registers and takes from them the chunk's maximum
-// and sum of exponentials and its `beams` largest logits: the beams-th largest
-// of the threads' own maxima bounds them from below (the warps sort theirs and
-// rank them in each other's lists), so only candidates at or above it (beams to
-// 32 * beams of kChunk) are ranked, by counting.  A second
-// launch joins a group's chunks: the log sums in 64 bits, then the best
-// continuations by the same ranking, on 64-bit scores.
+// One pass over the logits, bound by HBM (4 bytes a candidate): a warp takes a
+// strip of kStrip consecutive logits of a row and leaves its maximum and its sum
+// of exponentials, nothing else; no barrier, no shared memory, no list. A second
+// launch, one CTA per group, makes the rows' log sums (in 64 bits) and from them
+// every strip's best score. At most `beams` strips can hold a winner: those first
+// in the order (best score, then row and strip). Only they are read again, by a
+// warp each, and their `beams` best logits ranked by counting.
 //
-// Order: within a row by logit, ties to the lower token (the row's constant
-// shifts all alike); across rows by the 64-bit score, ties to the lower beam.
-// Every comparison is on unique (value, index) pairs, so the result does not
-// depend on the order in which candidates arrive.
+// Order: by the 64-bit score, ties to the lower row, then the lower token; equal
+// logits of one row have equal scores. Every comparison is on unique pairs, so
+// the result does not depend on the order in which warps arrive. A strip that is
+// not among the first `beams` holds no winner: each of those has a continuation
+// that comes before all of its own.
 #include "g4_common.cuh"
 #include "g4_kv.h"
 
+#include <cfloat>
+
 namespace g4 {
 
-constexpr int kBeamThreads = 256;
-constexpr int kBeamPer = 32;                          // logits per thread
-constexpr int kChunk = kBeamThreads * kBeamPer;
+constexpr int kScanThreads = 128;
+constexpr int kStrip = 1024;  // logits per warp: 32 per lane, 4 KB in flight
 constexpr int kMaxBeams = 32;
-constexpr int kBeamJoinThreads = 512;
+constexpr int kPickThreads = 512;
 
-// A float's order as an unsigned word (NaN below everything).
+// exp(v) is taken as 2^(v * kLog2e) with this rounded constant throughout, and
+// the logarithm divided by the same one, so its rounding does not enter.
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A strip: its largest logit m (-inf: none) and the sum of 2^(v * kLog2e - m * kLog2e).
+struct StripStat {
+  float m, sum;
+};
+
+// A number's order as an unsigned word (NaN below everything).
 __device__ __forceinline__ uint32_t order_of(float v) {
   if (!(v == v)) return 0u;
   const uint32_t u = __float_as_uint(v);
@@ -34,242 +44,286 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
+__device__ __forceinline__ unsigned long long order_of(double v) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
 
-struct ChunkStat {
-  float m, sum;
+__device__ __forceinline__ float beam_exp2(float x) {  // relative error 2^-22
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A strip's logits, 32 per lane (-inf behind the row's end); returns how lane
+// elements map to tokens: first + step * i, in runs of four where the row is
+// 16-byte aligned.
+struct StripMap {
+  int base, quad;
+  __device__ __forceinline__ int token(int i) const { return quad ? base + (i >> 2) * 128 + (i & 3) : base + i * 32; }
+};
+__device__ __forceinline__ StripMap load_strip(const float* row, int vocab, int t0, int lane, float (&v)[32]) {
+  const float* x = row + t0;
+  StripMap map;
+  map.quad = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  map.base = t0 + (map.quad ? 4 * lane : lane);
+  if (map.quad && t0 + kStrip <= vocab) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(x) + i * 32 + lane);
+      v[4 * i] = f.x;
+      v[4 * i + 1] = f.y;
+      v[4 * i + 2] = f.z;
+      v[4 * i + 3] = f.w;
+    }
+  } else {
+    map.quad = 0;
+    map.base = t0 + lane;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = map.base + 32 * i < vocab ? __ldg(x + lane + 32 * i) : -INFINITY;
+  }
+  return map;
+}
+
+__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const float* logits, long long stride, int vocab,
+                                                                 const int32_t* finished, int n_rows, int strips,
+                                                                 StripStat* stats) {
+  const int lane = threadIdx.x & 31;
+  const unsigned w = blockIdx.x * (kScanThreads / 32) + (threadIdx.x >> 5);
+  grid_dep_launch();
+  const unsigned row = w / (unsigned)strips;
+  if (row >= (unsigned)n_rows || (finished && finished[row])) return;  // a finished row needs no logits
+  float v[32];
+  load_strip(logits + (long long)row * stride, vocab, (int)(w - row * strips) * kStrip, lane, v);
+  float m0 = -INFINITY, m1 = -INFINITY;  // (a NaN is never the larger one)
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) {
+    m0 = fmaxf(m0, v[i]);
+    m1 = fmaxf(m1, v[i + 1]);
+  }
+  const float m = value_of(__reduce_max_sync(0xffffffffu, order_of(fmaxf(m0, m1))));
+  const float c = m == -INFINITY ? 0.f : __fmul_rn(m, kLog2e);
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i & 3] += beam_exp2(fmaf(v[i], kLog2e, -c));
+  float sum = (s[0] + s[1]) + (s[2] + s[3]);
+  if (!(sum == sum)) {  // NaNs count as masked
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) sum += v[i] == v[i] ? beam_exp2(fmaf(v[i], kLog2e, -c)) : 0.f;
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) stats[w] = StripStat{m, sum};
+}
+
+// A continuation's or strip's place in the order: larger key first, then lower index.
+struct __align__(16) Ranked {
+  unsigned long long key;  // 0: none
+  long long at;
+  __device__ __forceinline__ bool before(const Ranked& o) const {
+    return (key > o.key) | ((key == o.key) & (at < o.at));
+  }
 };
 
-// The lanes' keys in descending order (bitonic).
-__device__ __forceinline__ unsigned long long warp_sort(unsigned long long k, int lane) {
+// How many of n entries (shared memory) come before one; a warp together.
+__device__ __forceinline__ int warp_rank(const Ranked* all, int n, const Ranked& r, int lane) {
+  int rank = 0;
+  for (int j = lane; j < n; j += 32) rank += all[j].before(r);
+  return (int)__reduce_add_sync(0xffffffffu, (unsigned)rank);
+}
+
+// The lanes' entries in order (bitonic).
+__device__ __forceinline__ Ranked warp_sort(Ranked r, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
     for (int o = size >> 1; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-      const bool keep_max = ((lane & o) == 0) == ((lane & size) == 0);
-      k = (other > k) == keep_max ? other : k;
+      Ranked other;
+      other.key = __shfl_xor_sync(0xffffffffu, r.key, o);
+      other.at = __shfl_xor_sync(0xffffffffu, (int)r.at, o);
+      const bool keep_first = ((lane & o) == 0) == ((lane & size) == 0);
+      if (other.before(r) == keep_first) r = other;
     }
-  return k;
+  return r;
 }
 
-__global__ void __launch_bounds__(kBeamThreads, 4)
-    beam_chunk_kernel(const float* logits, long long stride, int vocab, const int32_t* finished, int beams, int chunks,
-                      unsigned long long* best, ChunkStat* stats) {
-  constexpr int NW = kBeamThreads / 32, G = kBeamPer / 4;
-  __shared__ unsigned long long top[NW][kMaxBeams];
-  __shared__ unsigned long long cand[kMaxBeams * kBeamPer];
-  __shared__ unsigned long long bound_s;
-  __shared__ float red[NW];
-  __shared__ int count;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
-  grid_dep_launch();
-  if (finished && finished[row]) return;  // its one continuation needs no logits
-  const float* x = logits + row * stride;
-  const int t0 = c * kChunk;
-  if (tid == 0) count = 0;
-  // group i of a thread: tokens t0 + i * 1024 + 4 tid + {0..3}
-  float v[G][4];
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && t0 + kChunk <= vocab;
-  if (vec) {
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + t0 + (i * kBeamThreads + tid) * 4));
-      v[i][0] = f.x;
-      v[i][1] = f.y;
-      v[i][2] = f.z;
-      v[i][3] = f.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < G; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = t0 + (i * kBeamThreads + tid) * 4 + j;
-        v[i][j] = t < vocab ? x[t] : -INFINITY;
-      }
-  }
-  // the thread's largest logit (a NaN is never the larger one) and its group
-  float m = -INFINITY;
-  int at = 0;
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const float g = fmaxf(fmaxf(v[i][0], v[i][1]), fmaxf(v[i][2], v[i][3]));
-    if (g > m) {
-      m = g;
-      at = i;
-    }
-  }
-  auto key_of = [&](float f, int token) {
-    return ((unsigned long long)order_of(f) << 32) | (0xffffffffu - (uint32_t)token);
-  };
-  // The bound: the beams-th largest of the threads' keys, a key being the
-  // largest logit with its group's last token, so at most that of the logit
-  // itself: beams candidates reach it, all in threads whose keys do.
-  const unsigned long long mine = key_of(m, t0 + (at * kBeamThreads + tid) * 4 + 3);
-  const unsigned long long sorted = warp_sort(mine, lane);
-  if (lane < beams) top[warp][lane] = sorted;
-  const float warp_max = value_of((uint32_t)(__shfl_sync(0xffffffffu, sorted, 0) >> 32));
-  if (lane == 0) red[warp] = warp_max;
-  __syncthreads();
-  float M = red[0];
-#pragma unroll
-  for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
-  if (lane < beams) {
-    int rank = lane;
-    for (int w = 1; w < NW; ++w) {  // in another warp's list: how many are larger
-      const unsigned long long* list = top[(warp + w) % NW];
-      int r = 0;
-      for (int i = 0; i < beams && list[i] > sorted; ++i) ++r;
-      rank += r;
-    }
-    if (rank == beams - 1) bound_s = sorted;
-  }
-  const float base = M == -INFINITY ? 0.f : M;
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    s0 += __expf(v[i][0] - base) + __expf(v[i][1] - base);
-    s1 += __expf(v[i][2] - base) + __expf(v[i][3] - base);
-  }
-  if (!(s0 + s1 == s0 + s1)) {  // NaNs count as masked
-    s0 = s1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < G; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s0 += v[i][j] == v[i][j] ? __expf(v[i][j] - base) : 0.f;
-  }
-  const float sum = warp_sum(s0 + s1);
-  __syncthreads();
-  if (lane == 0) red[warp] = sum;
-  const unsigned long long bound = bound_s;
-  if (mine >= bound) {
-    const float bv = value_of((uint32_t)(bound >> 32));
-#pragma unroll
-    for (int i = 0; i < G; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (v[i][j] >= bv) {
-          const unsigned long long k = key_of(v[i][j], t0 + (i * kBeamThreads + tid) * 4 + j);
-          if (k >= bound) cand[atomicAdd(&count, 1)] = k;
-        }
-  }
-  __syncthreads();
-  const int n = count;
-  unsigned long long* out = best + ((long long)row * chunks + c) * beams;
-  for (int i = tid; i < n; i += kBeamThreads) {
-    const unsigned long long k = cand[i];
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += cand[j] > k;
-    if (r < beams) out[r] = k;
-  }
-  if (tid == 0) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) t += red[i];
-    stats[(long long)row * chunks + c] = ChunkStat{M, t};
-  }
-}
-
-// A 64-bit score's order as an unsigned word.
-__device__ __forceinline__ unsigned long long order_of(double v) {
-  const long long u = __double_as_longlong(v);
-  return u < 0 ? ~(unsigned long long)u : (unsigned long long)u | 0x8000000000000000ull;
-}
-
-// One CTA per group: the rows' log sums, their best tokens over the chunks,
-// and the group's best continuations.
-__global__ void __launch_bounds__(kBeamJoinThreads) beam_join_kernel(
-    const unsigned long long* best, const ChunkStat* stats, const float* scores, const int32_t* finished, int beams,
-    int chunks, int pad_token, float* new_scores, int32_t* parents, int32_t* tokens) {
-  __shared__ double lse[kMaxBeams];
-  __shared__ unsigned long long row_key[kMaxBeams][kMaxBeams];  // a row's best logits, in order
-  __shared__ unsigned long long cand_key[kMaxBeams * kMaxBeams];
+__global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
+    const float* logits, long long stride, int vocab, const StripStat* stats, const float* scores,
+    const int32_t* finished, int beams, int strips, int pad_token, float* new_scores, int32_t* parents,
+    int32_t* tokens) {
+  constexpr int NW = kPickThreads / 32;
+  __shared__ double lse[kMaxBeams], score_of[kMaxBeams];
+  __shared__ int done[kMaxBeams];
+  __shared__ Ranked lists[NW * kMaxBeams];
+  __shared__ Ranked chosen[kMaxBeams];
+  __shared__ Ranked cand[kMaxBeams * kMaxBeams];  // at: row and token; until they are scored, key: the logit's order
   __shared__ double cand_score[kMaxBeams * kMaxBeams];
-  __shared__ int cand_row[kMaxBeams * kMaxBeams], cand_token[kMaxBeams * kMaxBeams];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, NW = kBeamJoinThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g0 = blockIdx.x * beams;
+  if (tid < beams) {
+    done[tid] = finished ? finished[g0 + tid] : 0;
+    score_of[tid] = (double)scores[g0 + tid];
+  }
+  __syncthreads();
   grid_dep_wait();
   for (int b = warp; b < beams; b += NW) {
-    const int row = g0 + b;
-    if (finished && finished[row]) continue;
-    const ChunkStat* st = stats + (long long)row * chunks;
-    const unsigned long long* list = best + (long long)row * chunks * beams;
-    // the row's best: sorted blocks of 32 keys, the lists' heads first; a block
-    // is looked at only if it can hold one of the best so far
-    unsigned long long kept = 0;  // lane i: the i-th largest so far
-    const int total = chunks * beams;
+    if (done[b]) continue;
+    const StripStat* st = stats + (long long)(g0 + b) * strips;
     float M = -INFINITY;
-    for (int i = lane; i < chunks; i += 32) M = fmaxf(M, st[i].m);
-    for (int i0 = 0; i0 < total; i0 += 32) {
-      // element i of this order: head i / chunks of chunk i % chunks
-      const int i = i0 + lane, head = i / chunks;
-      unsigned long long k = i < total ? list[(long long)(i - head * chunks) * beams + head] : 0;
-      const unsigned long long least = __shfl_sync(0xffffffffu, kept, beams - 1);
-      if (!__any_sync(0xffffffffu, k > least)) continue;
-      k = warp_sort(k, lane);
-      // both lists descend: the larger of element i and element 31 - i of the other are the 32 largest
-      const unsigned long long other = __shfl_sync(0xffffffffu, k, 31 - lane);
-      kept = warp_sort(other > kept ? other : kept, lane);
-    }
-    if (lane < beams) row_key[b][lane] = kept;
+    double s = 0.0;
+    // up to eight strips per lane stay in registers
+    constexpr int kHold = 8;
+    StripStat x[kHold];
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) x[i] = lane + 32 * i < strips ? st[lane + 32 * i] : StripStat{-INFINITY, 0.f};
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) M = fmaxf(M, x[i].m);
+    for (int i = lane + 32 * kHold; i < strips; i += 32) M = fmaxf(M, st[i].m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    double s = 0.0;
-    for (int i = lane; i < chunks; i += 32)
-      if (st[i].m > -INFINITY) s += (double)(st[i].sum * expf(st[i].m - M));
+    const float C = __fmul_rn(M, kLog2e);
+    auto part = [&](const StripStat& t) {
+      return t.m > -INFINITY ? t.sum * beam_exp2(__fmul_rn(t.m, kLog2e) - C) : 0.f;
+    };
+    float near = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) near += part(x[i]);
+    for (int i = lane + 32 * kHold; i < strips; i += 32) s += (double)part(st[i]);
+    s += (double)near;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) lse[b] = M == -INFINITY ? INFINITY : (double)M + log(s);
+    if (lane == 0) lse[b] = M == -INFINITY ? INFINITY : ((double)C + log2(s)) / (double)kLog2e;
   }
   __syncthreads();
-  const int n = beams * beams;
-  for (int i = tid; i < n; i += kBeamJoinThreads) {
-    const int b = i / beams, k = i - b * beams, row = g0 + b;
-    double sc = -INFINITY;
-    int token = -1;
-    if (finished && finished[row]) {
-      if (k == 0) {
-        sc = (double)scores[row];
-        token = pad_token;
+
+  // ---- the strips in order of their best score: each warp's first ones, then all
+  Ranked kept{0, 0x7fffffff};
+  const int total = beams * strips;
+  for (int i0 = warp * 32; i0 < total; i0 += kPickThreads) {
+    const int i = i0 + lane, b = min(i / strips, beams - 1);
+    Ranked r{0, i};
+    if (i < total) {
+      double sc = -INFINITY;
+      if (done[b]) {
+        if (i == b * strips) sc = score_of[b];
+      } else {
+        const float m = stats[(long long)g0 * strips + i].m;
+        if (m > -INFINITY) sc = score_of[b] + ((double)m - lse[b]);
       }
-    } else {
-      const unsigned long long key = row_key[b][k];
-      const float v = value_of((uint32_t)(key >> 32));
-      if (v > -INFINITY) {
-        sc = (double)scores[row] + ((double)v - lse[b]);
-        token = (int)(0xffffffffu - (uint32_t)key);
-      }
+      if (sc > -INFINITY) r.key = order_of(sc);
     }
-    if (!(sc == sc)) sc = -INFINITY;
-    cand_score[i] = sc;
-    cand_row[i] = row;
-    cand_token[i] = token;
-    cand_key[i] = order_of(sc);
+    const unsigned long long least = __shfl_sync(0xffffffffu, kept.key, beams - 1);
+    if (!__any_sync(0xffffffffu, r.key > least)) continue;
+    r = warp_sort(r, lane);
+    if (__all_sync(0xffffffffu, kept.key == 0)) {  // the warp's first
+      kept = r;
+      continue;
+    }
+    // both are in order: of entry i and entry 31 - i of the other, the first are the 32 first
+    Ranked other;
+    other.key = __shfl_sync(0xffffffffu, r.key, 31 - lane);
+    other.at = __shfl_sync(0xffffffffu, (int)r.at, 31 - lane);
+    if (other.before(kept)) kept = other;
+    kept = warp_sort(kept, lane);
+  }
+  if (lane < beams) lists[warp * beams + lane] = kept;
+  if (tid < beams) chosen[tid] = Ranked{0, 0};
+  __syncthreads();
+  for (int i = warp; i < NW * beams; i += NW) {
+    const Ranked r = lists[i];
+    if (r.key == 0) continue;
+    const int rank = warp_rank(lists, NW * beams, r, lane);
+    if (rank < beams && lane == 0) chosen[rank] = r;
   }
   __syncthreads();
-  // rank by (score, then beam and token order); i is in beam order, and in
-  // token order where a beam's scores tie
-  for (int i = tid; i < n; i += kBeamJoinThreads) {
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += cand_key[j] > cand_key[i] || (cand_key[j] == cand_key[i] && j < i);
-    if (r < beams) {
-      const bool live = cand_score[i] > -INFINITY;
-      new_scores[g0 + r] = live ? (float)cand_score[i] : -INFINITY;
-      parents[g0 + r] = live ? cand_row[i] : -1;
-      tokens[g0 + r] = live ? cand_token[i] : -1;
+
+  // ---- their best logits: a warp per strip
+  for (int r = warp; r < beams; r += NW) {
+    const Ranked strip = chosen[r];
+    const int b = min((int)strip.at / strips, beams - 1), row = g0 + b;
+    float v[32];
+    StripMap map{0, 0};
+    const bool reads = strip.key != 0 && !done[b];  // the same in every lane
+    if (reads) map = load_strip(logits + (long long)row * stride, vocab, ((int)strip.at - b * strips) * kStrip, lane, v);
+    // the lane's largest logit, lowest token first (its elements are in token
+    // order); taken, the lane looks for its next one
+    float m = -INFINITY;
+    int at = 0;
+    auto look = [&]() {
+      float x[16];
+      int i_of[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool second = v[2 * i + 1] > v[2 * i] || !(v[2 * i] == v[2 * i]);
+        x[i] = second ? v[2 * i + 1] : v[2 * i];
+        i_of[i] = 2 * i + second;
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+          const bool second = x[2 * i + 1] > x[2 * i] || !(x[2 * i] == x[2 * i]);
+          x[i] = second ? x[2 * i + 1] : x[2 * i];
+          i_of[i] = second ? i_of[2 * i + 1] : i_of[2 * i];
+        }
+      m = x[0];
+      at = i_of[0];
+    };
+    if (reads) look();
+    for (int k = 0; k < beams; ++k) {
+      const uint32_t mine = m > -INFINITY ? order_of(m) : 0u;
+      const uint32_t top = __reduce_max_sync(0xffffffffu, mine);
+      const uint32_t token = (uint32_t)map.token(at);
+      const uint32_t first = __reduce_min_sync(0xffffffffu, top && mine == top ? token : 0xffffffffu);
+      if (lane == 0) cand[r * beams + k] = Ranked{top, ((long long)row << 32) | first};
+      if (top && mine == top && token == first) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i == at) v[i] = -INFINITY;
+        look();
+      }
+      __syncwarp();
+    }
+    if (lane == 0 && strip.key != 0 && !reads) cand[r * beams] = Ranked{1, ((long long)row << 32) | (uint32_t)pad_token};
+  }
+  if (tid < beams) {
+    new_scores[g0 + tid] = -INFINITY;
+    parents[g0 + tid] = -1;
+    tokens[g0 + tid] = -1;
+  }
+  __syncthreads();
+
+  // ---- their scores, and the first of all
+  const int n = beams * beams;
+  for (int i = tid; i < n; i += kPickThreads) {
+    const Ranked c = cand[i];
+    if (c.key == 0) continue;
+    const int b = (int)(c.at >> 32) - g0;
+    const double sc = done[b] ? score_of[b] : score_of[b] + ((double)value_of((uint32_t)c.key) - lse[b]);
+    cand_score[i] = sc;
+    cand[i].key = order_of(sc);
+  }
+  __syncthreads();
+  for (int i = warp; i < n; i += NW) {
+    const Ranked c = cand[i];
+    if (c.key == 0) continue;
+    const int rank = warp_rank(cand, n, c, lane);
+    if (rank < beams && lane == 0) {
+      new_scores[g0 + rank] = (float)cand_score[i];
+      parents[g0 + rank] = (int)(c.at >> 32);
+      tokens[g0 + rank] = (int)(uint32_t)c.at;
     }
   }
 }
 
 int beam_prepare() {
   cudaFuncAttributes fa;
-  cudaError_t e = cudaFuncGetAttributes(&fa, beam_chunk_kernel);
-  if (!e) e = cudaFuncGetAttributes(&fa, beam_join_kernel);
+  cudaError_t e = cudaFuncGetAttributes(&fa, beam_scan_kernel);
+  if (!e) e = cudaFuncGetAttributes(&fa, beam_pick_kernel);
   return e;
 }
 
-static long long beam_chunks(int vocab) { return ((long long)vocab + kChunk - 1) / kChunk; }
+static long long beam_strips(int vocab) { return ((long long)vocab + kStrip - 1) / kStrip; }
 
 }  // namespace g4
 
@@ -279,15 +333,16 @@ extern "C" {
 
 size_t g4_beam_select_workspace(int n_rows, int vocab, int beams) {
   if (n_rows < 1 || vocab < 1 || vocab > (1 << 30) || beams < 1 || beams > kMaxBeams) return 0;
-  return (size_t)n_rows * beam_chunks(vocab) * (beams * 8 + sizeof(ChunkStat));
+  return (size_t)n_rows * beam_strips(vocab) * sizeof(StripStat);
 }
 
 int g4_beam_select(g4_ctx* c, const float* logits, int64_t stride, int vocab, const float* scores,
                    const int32_t* finished, int n_rows, int beams, int pad_token, float* new_scores, int32_t* parents,
                    int32_t* tokens, void* work, size_t work_bytes, void* stream) {
   if (!c) return G4_E_ARG;
-  const long long chunks = vocab > 0 ? beam_chunks(vocab) : 0;
-  if (n_rows < 0 || vocab < 1 || vocab > (1 << 30) || beams < 1 || beams > kMaxBeams || n_rows % beams || n_rows * chunks > 0x7fffffffll ||
+  const long long strips = vocab > 0 ? beam_strips(vocab) : 0;
+  if (n_rows < 0 || vocab < 1 || vocab > (1 << 30) || beams < 1 || beams > kMaxBeams || n_rows % beams ||
+      n_rows * strips > (1ll << 30) ||
       (n_rows > 0 && (!logits || !scores || !new_scores || !parents || !tokens || (n_rows > 1 && stride < vocab)))) {
     c->set_err("g4_beam_select: bad arguments (%d rows of %d tokens, %d beams, at most %d; rows a multiple of the "
                "beams)", n_rows, vocab, beams, kMaxBeams);
@@ -303,14 +358,13 @@ int g4_beam_select(g4_ctx* c, const float* logits, int64_t stride, int vocab, co
   DeviceScope scope(c);
   if (scope.rc) return scope.rc;
   cudaStream_t st = (cudaStream_t)stream;
-  unsigned long long* best = static_cast<unsigned long long*>(work);
-  ChunkStat* stats = reinterpret_cast<ChunkStat*>(best + (size_t)n_rows * chunks * beams);
-  beam_chunk_kernel<<<(unsigned)(n_rows * chunks), kBeamThreads, 0, st>>>(logits, stride, vocab, finished, beams,
-                                                                          (int)chunks, best, stats);
+  StripStat* stats = static_cast<StripStat*>(work);
+  const unsigned grid = (unsigned)((n_rows * strips + kScanThreads / 32 - 1) / (kScanThreads / 32));
+  beam_scan_kernel<<<grid, kScanThreads, 0, st>>>(logits, stride, vocab, finished, n_rows, (int)strips, stats);
   cudaError_t e = cudaGetLastError();
   if (!e)
-    e = launch_after(beam_join_kernel, dim3(n_rows / beams), dim3(kBeamJoinThreads), 0, st, best, stats, scores,
-                     finished, beams, (int)chunks, pad_token, new_scores, parents, tokens);
+    e = launch_after(beam_pick_kernel, dim3(n_rows / beams), dim3(kPickThreads), 0, st, logits, stride, vocab, stats,
+                     scores, finished, beams, (int)strips, pad_token, new_scores, parents, tokens);
   return e ? c->cuda_fail(e, "g4_beam_select") : 0;
 }
 

@@ -80,7 +80,7 @@ def test_beam_arguments_refused(g4, fake):
                dict(stride=9), dict(x=None), dict(work=None), dict(size=8)]:
         assert call(**kw) == -1, kw
     assert L.g4_beam_select_workspace(0, 10, 2) == 0 and L.g4_beam_select_workspace(4, 10, 33) == 0
-    assert L.g4_beam_select_workspace(4, 8193, 2) == 4 * 2 * (2 * 8 + 8)
+    assert L.g4_beam_select_workspace(4, 1025, 2) == 4 * 2 * 8
 
 
 def test_python_layer_checks_tensors(g4):

@@ -476,7 +476,7 @@ def check_beams(g4, ctx, logits, scores, beams, finished=None, pad=0):
     assert np.all(abs(s[live] - want[0][live]) <= 2.0 ** -18 + 2.0 ** -24 * abs(want[0][live]))
 
 
-@pytest.mark.parametrize("vocab", [1, 3, 255, 8191, 8192, 8193, 32001, 262144])
+@pytest.mark.parametrize("vocab", [1, 3, 255, 1023, 1024, 1025, 8192, 32001, 262144])
 @pytest.mark.parametrize("groups,beams", [(1, 1), (3, 4), (2, 7), (1, 32)])
 def test_beam_select(g4, ctx, vocab, groups, beams):
     rng = np.random.default_rng(vocab + beams)
@@ -512,6 +512,18 @@ def test_beam_masks_and_finished(g4, ctx):
     low = np.full((4, 300), np.finfo(np.float32).min, np.float32)  # the type's lowest value masks, too
     low[:, 7] = 1.0
     check_beams(g4, ctx, low, np.zeros(4, np.float32), 4)
+
+
+@pytest.mark.parametrize("beams", [1, 5, 32])
+def test_beam_ordered_logits(g4, ctx, beams):
+    """Rows that rise, fall or stay level over the vocabulary: every piece of a
+    rising row beats all before it, at once or within a few."""
+    vocab = 100003
+    up = np.linspace(-10, 10, vocab).astype(np.float32)
+    saw = (up + np.where(np.arange(vocab) % 7 == 0, 3.0, 0.0)).astype(np.float32)
+    rows = np.stack([up, up[::-1], np.zeros(vocab, np.float32), saw, np.round(up), np.where(up > 9.9, up, -np.inf)])
+    rows = np.repeat(rows, beams, axis=0).astype(np.float32)
+    check_beams(g4, ctx, rows, np.tile(-np.arange(beams) * 0.125, 6).astype(np.float32), beams)
 
 
 def test_beam_strided_and_in_place(g4, ctx):
