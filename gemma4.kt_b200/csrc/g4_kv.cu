@@ -24,7 +24,7 @@
 namespace g4 {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kForkThreads = 256;
+constexpr int kForkThreads = 1024;
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 8;
 
@@ -40,38 +40,66 @@ static KvDev kv_dev(const g4_kv* kv) {
 }
 
 // Exclusive prefix sum over the CTA (kPlanThreads threads); total in *sum.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* sum) {
+// Callers alternate between two sets of warp_sums, so that one barrier is enough.
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, T* warp_sums, T* sum) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = v;
+  T x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  __syncthreads();
   if (lane == 31) warp_sums[w] = x;
   __syncthreads();
-  if (w == 0) {
-    int s = warp_sums[lane];
+  const T mine = warp_sums[lane];
+  T s = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    warp_sums[lane] = s;
+  for (int o = 1; o < 32; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
   }
-  __syncthreads();
-  *sum = warp_sums[31];
-  return x - v + (w ? warp_sums[w - 1] : 0);
+  *sum = __shfl_sync(0xffffffffu, s, 31);
+  return x - v + __shfl_sync(0xffffffffu, s - mine, w);
 }
 
 __device__ __forceinline__ bool page_ok(int p, int n_pages) { return (unsigned)p < (unsigned)n_pages; }
 
-// Pages a thread owns in the scans below: consecutive ones, so that one block
-// scan gives every thread the rank of its first page.
-__device__ __forceinline__ int pages_per_thread(int n_pages) {
-  return ((n_pages + kPlanThreads - 1) / kPlanThreads + 3) / 4 * 4;
-}
+// The pages a thread owns in the scans: kRun consecutive ones per round of the
+// CTA, in registers between counting and ranking while one round covers the pool.
+constexpr int kRun = 8;
+struct PageRun {
+  int refs[kRun];
+  int first, n_pages;
+  __device__ __forceinline__ void load(const int32_t* r, int round, int n) {
+    n_pages = n;
+    first = (round * kPlanThreads + threadIdx.x) * kRun;
+    if (first + kRun <= n) {
+      const int4 x = __ldcg(reinterpret_cast<const int4*>(r + first));
+      const int4 y = __ldcg(reinterpret_cast<const int4*>(r + first) + 1);
+      refs[0] = x.x, refs[1] = x.y, refs[2] = x.z, refs[3] = x.w;
+      refs[4] = y.x, refs[5] = y.y, refs[6] = y.z, refs[7] = y.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) refs[j] = first + j < n ? __ldcg(r + first + j) : 0;
+    }
+  }
+  __device__ __forceinline__ bool used(int j) const { return refs[j] > 0; }
+  __device__ __forceinline__ bool free(int j) const { return refs[j] <= 0 && first + j < n_pages; }
+  __device__ __forceinline__ int count_used() const {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) c += used(j);
+    return c;
+  }
+  __device__ __forceinline__ int count_free() const {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) c += free(j);
+    return c;
+  }
+};
+__device__ __forceinline__ int page_rounds(int n_pages) { return (n_pages + kPlanThreads * kRun - 1) / (kPlanThreads * kRun); }
 
 // g4_kv_resize, planning: new lengths for the entries' sequences, pages given
 // back and taken, and the list of shared last pages to copy.
@@ -86,12 +114,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
   int* el = en + n;             // shared-page candidate: the last, partly filled page (-1: none)
   int* ec = el + n;             // 1: that page is copied
   int* ea = ec + n;             // first of the entry's pages in free_list
-  __shared__ int warp_sums[32];
+  __shared__ long long sums64[2][32];
+  __shared__ int sums[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ps = d.page_size;
   grid_dep_launch();
+  PageRun run;
+  run.load(d.refs, 0, d.n_pages);  // looked at below, again if pages are given back
   for (int i = tid; i < d.n_seqs; i += kPlanThreads) owner[i] = 0x7fffffff;
   __syncthreads();
   unsigned bad = 0;
+  int shrinks = 0;
   for (int i = tid; i < n; i += kPlanThreads) {
     int s = seqs[i];
     const int nl = new_lens[i];
@@ -115,6 +147,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
       continue;
     }
     eo[i] = old;
+    shrinks |= en[i] < old;
     if (en[i] > old && old % ps != 0) {
       const int last = d.table[(size_t)s * d.max_pages + old / ps];
       if (page_ok(last, d.n_pages)) {
@@ -125,57 +158,64 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
       }
     }
   }
-  __syncthreads();
-  // sequences that shrink give pages back first
-  for (int i = warp; i < n; i += kPlanThreads / 32) {
-    if (es[i] < 0 || en[i] >= eo[i]) continue;
-    const int32_t* row = d.table + (size_t)es[i] * d.max_pages;
-    for (int p = (en[i] + ps - 1) / ps + lane; p < (eo[i] + ps - 1) / ps; p += 32)
-      if (page_ok(row[p], d.n_pages)) atomicSub(d.refs + row[p], 1);
+  shrinks = __syncthreads_or(shrinks);
+  if (shrinks) {  // sequences that shrink give pages back first
+    for (int i = warp; i < n; i += kPlanThreads / 32) {
+      if (es[i] < 0 || en[i] >= eo[i]) continue;
+      const int32_t* row = d.table + (size_t)es[i] * d.max_pages;
+      for (int p = (en[i] + ps - 1) / ps + lane; p < (eo[i] + ps - 1) / ps; p += 32)
+        if (page_ok(row[p], d.n_pages)) atomicSub(d.refs + row[p], 1);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   // a shared last page is copied by every sequence that grows into it, except
   // one that is left as its only holder; pages wanted per entry
-  int base = 0, cbase = 0;
-  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+  // (both sums in one scan: pages in the low, copies in the high half)
+  long long base = 0;
+  for (int i0 = 0, round = 0; i0 < n; i0 += kPlanThreads, ++round) {
     const int i = i0 + tid;
     int need = 0, copied = 0;
     if (i < n && es[i] >= 0) {
       if (el[i] >= 0) {
-        int earlier = 0;
-        for (int j = 0; j < i; ++j) earlier += el[j] == el[i];
-        copied = __ldcg(d.refs + el[i]) - earlier > 1;
+        const int held = __ldcg(d.refs + el[i]);
+        if (held > 1) {
+          int earlier = 0;
+          for (int j = 0; j < i; ++j) earlier += el[j] == el[i];
+          copied = held - earlier > 1;
+        }
       }
       const int more = (en[i] + ps - 1) / ps - (eo[i] + ps - 1) / ps;
       need = max(0, more) + copied;
     }
-    int sum;
-    const int at = block_scan(need, warp_sums, &sum);
+    long long sum;
+    const long long at = base + block_scan(((long long)copied << 32) | need, sums64[round & 1], &sum);
     if (i < n) {
-      ea[i] = base + at;
+      ea[i] = (int)at;
       ec[i] = copied;
     }
+    if (copied) moves[at >> 32] = KvMove{el[i], i, eo[i] % ps};  // dst: the entry, its page below
     base += sum;
-    int csum;
-    const int c = block_scan(copied, warp_sums, &csum);
-    if (copied) moves[cbase + c] = KvMove{el[i], i, eo[i] % ps};  // dst: the entry, its page below
-    cbase += csum;
   }
-  const int total = base;
+  const int total = (int)base, copies = (int)(base >> 32);
   // the lowest free pages
-  const int per = pages_per_thread(d.n_pages), p0 = tid * per, p1 = min(p0 + per, d.n_pages);
   int found = 0;
   if (total > 0) {
-    int mine = 0;
-    for (int p = p0; p < p1; ++p) mine += __ldcg(d.refs + p) <= 0;
-    int at = block_scan(mine, warp_sums, &found);
-    for (int p = p0; p < p1 && at < total; ++p)
-      if (__ldcg(d.refs + p) <= 0) free_list[at++] = p;
+    for (int round = 0; round < page_rounds(d.n_pages) && found < total; ++round) {
+      if (round || shrinks) run.load(d.refs, round, d.n_pages);
+      int sum, at = found + block_scan(run.count_free(), sums[round & 1], &sum);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j)
+        if (run.free(j)) {
+          if (at < total) free_list[at] = run.first + j;
+          ++at;
+        }
+      found += sum;
+    }
   }
   if (bad) atomicOr(d.flags, bad);
   __syncthreads();
   if (found < total) {  // nothing changes: take the given-back pages again
-    for (int i = warp; i < n; i += kPlanThreads / 32) {
+    for (int i = shrinks ? warp : n; i < n; i += kPlanThreads / 32) {
       if (es[i] < 0 || en[i] >= eo[i]) continue;
       const int32_t* row = d.table + (size_t)es[i] * d.max_pages;
       for (int p = (en[i] + ps - 1) / ps + lane; p < (eo[i] + ps - 1) / ps; p += 32)
@@ -188,7 +228,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
     return;
   }
   for (int k = tid; k < total; k += kPlanThreads) d.refs[free_list[k]] = 1;
-  for (int k = tid; k < cbase; k += kPlanThreads) {
+  for (int k = tid; k < copies; k += kPlanThreads) {
     const int i = moves[k].dst;
     moves[k].dst = free_list[ea[i]];
     atomicSub(d.refs + moves[k].src, 1);
@@ -202,7 +242,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
     for (int p = want + lane; p < have; p += 32) row[p] = -1;
     if (lane == 0) d.lens[es[i]] = en[i];
   }
-  if (tid == 0) plan[0] = cbase;
+  if (tid == 0) plan[0] = copies;
 }
 
 // g4_kv_fork: dst[i] holds the pages of src[i].  A CTA owns W columns of the
@@ -263,21 +303,36 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_kernel(KvDev d, const in
 // L moves to the k-th free page before L.
 __global__ void __launch_bounds__(kPlanThreads) kv_compact_kernel(KvDev d, int32_t* moved, KvMove* moves,
                                                                   int32_t* plan) {
-  __shared__ int warp_sums[32];
+  __shared__ int sums[2][32];
   grid_dep_launch();
-  const int tid = threadIdx.x, per = pages_per_thread(d.n_pages), p0 = tid * per, p1 = min(p0 + per, d.n_pages);
-  int mine = 0;
-  for (int p = p0; p < p1; ++p) mine += __ldcg(d.refs + p) > 0;
-  int L, holes;
-  int live = block_scan(mine, warp_sums, &L);  // live pages before p0
-  int gaps = 0;
-  for (int p = p0; p < min(p1, L); ++p) gaps += __ldcg(d.refs + p) <= 0;
-  int hole = block_scan(gaps, warp_sums, &holes);
-  for (int p = p0; p < p1; ++p) {
-    const bool used = __ldcg(d.refs + p) > 0;
-    if (p < L && !used) moves[hole++].dst = p;
-    if (p >= L && used) moves[live - (L - holes)].src = p;
-    live += used;
+  const int tid = threadIdx.x, rounds = page_rounds(d.n_pages);
+  PageRun run;
+  int L = 0, which = 0;
+  for (int round = 0; round < rounds; ++round) {
+    run.load(d.refs, round, d.n_pages);
+    int sum;
+    block_scan(run.count_used(), sums[which ^= 1], &sum);
+    L += sum;
+  }
+  // free pages before L take the live ones behind it: as many of one as of the other
+  int holes = 0, movers = 0;
+  for (int round = 0; round < rounds; ++round) {
+    if (rounds > 1) run.load(d.refs, round, d.n_pages);
+    int gaps = 0, late = 0;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      gaps += run.free(j) && run.first + j < L;
+      late += run.used(j) && run.first + j >= L;
+    }
+    int sum, hole = holes + block_scan(gaps, sums[which ^= 1], &sum);
+    holes += sum;
+    int mover = movers + block_scan(late, sums[which ^= 1], &sum);
+    movers += sum;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      if (run.free(j) && run.first + j < L) moves[hole++].dst = run.first + j;
+      if (run.used(j) && run.first + j >= L) moves[mover++].src = run.first + j;
+    }
   }
   __syncthreads();
   for (int k = tid; k < holes; k += kPlanThreads) {
@@ -340,10 +395,10 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(KvDev d, const Kv
 }
 
 __global__ void __launch_bounds__(kPlanThreads) kv_count_free_kernel(KvDev d) {
-  __shared__ int warp_sums[32];
+  __shared__ int sums[32];
   int mine = 0, sum;
   for (int p = threadIdx.x; p < d.n_pages; p += kPlanThreads) mine += d.refs[p] <= 0;
-  block_scan(mine, warp_sums, &sum);
+  block_scan(mine, sums, &sum);
   if (threadIdx.x == 0) d.flags[1] = (unsigned)sum;
 }
 
