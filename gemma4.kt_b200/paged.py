@@ -19,22 +19,29 @@ skipped and reported by KvCache.check().
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
-from ._lib import KvConfigStruct, KvQueriesStruct, KvRowsStruct, RopeConfigStruct, check, lib
+from ._lib import KvConfigStruct, RopeConfigStruct, check, lib
 from .floattensor import Context, GGMLType, UnsupportedOperation
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 
 
-def _stream(ctx: Context, stream):
+# g4_kv_rows and g4_kv_queries (include/g4.h), packed: a call's arguments are
+# built a few hundred nanoseconds faster than as ctypes structures.
+_ROWS = struct.Struct("@iiPPPPqqqqPPPPif")
+_QUERIES = struct.Struct("@iiPPqqPPfii4x")
+
+
+def _stream(device: int, stream):
     if stream is not None:
         return int(stream)
     import torch
 
-    return torch.cuda.current_stream(ctx.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device)  # torch.cuda.current_stream(device).cuda_stream
 
 
 def _workspace(ctx: Context, n: int, stream):
@@ -42,25 +49,34 @@ def _workspace(ctx: Context, n: int, stream):
     import torch
 
     if stream is None:
-        return torch.empty(n, dtype=torch.uint8, device=f"cuda:{ctx.device}")
+        return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
     with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=ctx.device)):
-        return torch.empty(n, dtype=torch.uint8, device=f"cuda:{ctx.device}")
+        return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
 
 
-def _tensor(ctx: Context, t, name: str, dtype, rows: int | None = None, width: int | None = None):
-    """Check a tensor of `rows` entries, or (width given) of rows x width with
-    any row stride; returns (address, floats between rows)."""
-    if not t.is_cuda or t.device.index != ctx.device:
-        raise ValueError(f"{name} must be a CUDA tensor on device {ctx.device}, got {t.device}")
+def _wrong(device: int, t, name: str, dtype, what: str):
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be a CUDA tensor on device {device}, got {t.device}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if width is None:
-        if (rows is not None and t.numel() != rows) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous with {rows} entries, got {tuple(t.shape)}")
-        return t.data_ptr(), 0
-    if t.dim() != 2 or t.shape[1] != width or t.shape[0] != rows or (width > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be [{rows}, {width}] with consecutive columns, got {tuple(t.shape)}")
-    return t.data_ptr(), t.stride(0)
+    raise ValueError(f"{name} must be {what}, got {tuple(t.shape)} with strides {t.stride()}")
+
+
+def _vector(device: int, t, name: str, dtype, n: int):
+    """Address of a contiguous tensor of n entries."""
+    if t.get_device() != device or t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        _wrong(device, t, name, dtype, f"contiguous with {n} entries")
+    return t.data_ptr()
+
+
+def _matrix(device: int, t, name: str, dtype, rows: int, width: int):
+    """Address of a [rows, width] tensor with consecutive columns, and the
+    entries between its rows."""
+    if t.get_device() == device and t.dtype == dtype and t.shape == (rows, width):
+        step, one = t.stride()
+        if one == 1 or width <= 1:
+            return t.data_ptr(), step
+    _wrong(device, t, name, dtype, f"[{rows}, {width}] with consecutive columns")
 
 
 class _Owner:
@@ -112,6 +128,7 @@ class Rope:
         check(rc, ctx.handle, "g4_rope_create")
         self.ctx, self.head_size, self.handle = ctx, head_size, h
         self._owner = _Owner(h, lib().g4_rope_free)
+        self._apply = lib().g4_rope_apply
 
     def free(self) -> None:
         self.handle = None
@@ -122,14 +139,16 @@ class Rope:
         [rows] (int32); out may be x; rows at negative positions stay."""
         import torch
 
+        dev = self.ctx.device
         rows, width = x.shape if x.dim() == 2 else (0, 0)
-        if x.dim() != 2 or width % self.head_size or not width:
+        if not width or width % self.head_size:
             raise ValueError(f"x must be [rows, heads * {self.head_size}], got {tuple(x.shape)}")
-        xp, xs = _tensor(self.ctx, x, "x", torch.float32, rows, width)
-        op, os_ = _tensor(self.ctx, out, "out", torch.float32, rows, width)
-        pp, _ = _tensor(self.ctx, pos, "pos", torch.int32, rows)
-        check(lib().g4_rope_apply(self.handle, xp, xs, op, os_, width // self.head_size, pp, rows,
-                                  _stream(self.ctx, stream)), self.ctx.handle, "g4_rope_apply")
+        xp, xs = _matrix(dev, x, "x", torch.float32, rows, width)
+        op, os_ = _matrix(dev, out, "out", torch.float32, rows, width)
+        pp = _vector(dev, pos, "pos", torch.int32, rows)
+        rc = self._apply(self.handle, xp, xs, op, os_, width // self.head_size, pp, rows, _stream(dev, stream))
+        if rc:
+            check(rc, self.ctx.handle, "g4_rope_apply")
 
 
 class KvCache:
@@ -157,6 +176,7 @@ class KvCache:
         self.max_positions, self.max_pages = max_positions, -(-max_positions // page_size)
         self._work = [lib().g4_kv_attend_workspace(h, l) for l in range(heads.size)]
         self._views = {}
+        self._lib = lib()
 
     def free(self) -> None:
         """Release the pages (no view of them is used afterwards)."""
@@ -213,35 +233,38 @@ class KvCache:
     def _pairs(self, fn, a, b, names, stream):
         import torch
 
-        n = a.numel()
-        ap, _ = _tensor(self.ctx, a, names[0], torch.int32, n)
-        bp, _ = _tensor(self.ctx, b, names[1], torch.int32, n)
-        check(getattr(lib(), fn)(self.handle, ap, bp, n, _stream(self.ctx, stream)), self.ctx.handle, fn)
+        dev, n = self.ctx.device, a.numel()
+        ap = _vector(dev, a, names[0], torch.int32, n)
+        bp = _vector(dev, b, names[1], torch.int32, n)
+        rc = fn(self.handle, ap, bp, n, _stream(dev, stream))
+        if rc:
+            check(rc, self.ctx.handle, fn.__name__)
 
     def resize(self, seqs, lens, stream=None) -> None:
         """Pages for lens[i] positions of sequence seqs[i] (int32 tensors; 0 frees
         it); a shared, partly filled last page is copied when a sequence grows
         into it.  Without enough free pages nothing changes (check())."""
-        self._pairs("g4_kv_resize", seqs, lens, ("seqs", "lens"), stream)
+        self._pairs(self._lib.g4_kv_resize, seqs, lens, ("seqs", "lens"), stream)
 
     def fork(self, src, dst, stream=None) -> None:
         """Sequence dst[i] shares the pages of src[i] as they were before the call
         (its own are given back); negative entries are padding."""
-        self._pairs("g4_kv_fork", src, dst, ("src", "dst"), stream)
+        self._pairs(self._lib.g4_kv_fork, src, dst, ("src", "dst"), stream)
 
     def copy_pages(self, src, dst, stream=None) -> None:
         """Whole pages src[i] -> dst[i] in every layer."""
-        self._pairs("g4_kv_copy_pages", src, dst, ("src", "dst"), stream)
+        self._pairs(self._lib.g4_kv_copy_pages, src, dst, ("src", "dst"), stream)
 
     def compact(self, stream=None) -> None:
         """Live pages to the front of the pool; the table follows."""
-        check(lib().g4_kv_compact(self.handle, _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_compact")
+        check(self._lib.g4_kv_compact(self.handle, _stream(self.ctx.device, stream)), self.ctx.handle, "g4_kv_compact")
 
     def check(self, stream=None) -> int:
         """Wait for the stream; raise what the cache's calls recorded, else the
         number of free pages."""
         n = C.c_int()
-        check(lib().g4_kv_check(self.handle, C.byref(n), _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_check")
+        check(self._lib.g4_kv_check(self.handle, C.byref(n), _stream(self.ctx.device, stream)), self.ctx.handle,
+              "g4_kv_check")
         return n.value
 
     # ---- rows
@@ -253,25 +276,28 @@ class KvCache:
         [rows, heads * head_size] with any row stride."""
         import torch
 
-        f32, n = torch.float32, pos.numel()
+        dev, f32, i32, n = self.ctx.device, torch.float32, torch.int32, pos.numel()
         if not 0 <= layer < len(self.head_size):
             raise ValueError(f"layer {layer} of {len(self.head_size)}")
         hs, width = self.head_size[layer], self.n_kv_heads[layer] * self.head_size[layer]
-        kp, ks = _tensor(self.ctx, k, "k", f32, n, width)
-        vp, vs = _tensor(self.ctx, v, "v", f32, n, width)
+        kp, ks = _matrix(dev, k, "k", f32, n, width)
+        vp, vs = _matrix(dev, v, "v", f32, n, width)
         heads = qp = qs = op = os_ = 0
         if q is not None:
-            if q.dim() != 2 or q.shape[1] % hs or not q.shape[1]:
+            wide = q.shape[-1]
+            heads = wide // hs
+            if not heads or heads * hs != wide:
                 raise ValueError(f"q must be [rows, heads * {hs}], got {tuple(q.shape)}")
-            heads = q.shape[1] // hs
-            qp, qs = _tensor(self.ctx, q, "q", f32, n, q.shape[1])
-            op, os_ = _tensor(self.ctx, q_out, "q_out", f32, n, q.shape[1])
-        norms = [_tensor(self.ctx, w, "norm weight", f32, hs)[0] if w is not None else None for w in (q_norm, k_norm)]
-        rows = KvRowsStruct(n, heads, qp or None, kp, vp, op or None, qs, ks, vs, os_,
-                            _tensor(self.ctx, seqs, "seqs", torch.int32, n)[0],
-                            _tensor(self.ctx, pos, "pos", torch.int32, n)[0], *norms, int(bool(v_norm)), eps)
-        check(lib().g4_kv_append(self.handle, layer, C.byref(rows), rope.handle if rope is not None else None,
-                                 _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_append")
+            qp, qs = _matrix(dev, q, "q", f32, n, wide)
+            op, os_ = _matrix(dev, q_out, "q_out", f32, n, wide)
+        rows = _ROWS.pack(n, heads, qp, kp, vp, op, qs, ks, vs, os_, _vector(dev, seqs, "seqs", i32, n),
+                          _vector(dev, pos, "pos", i32, n),
+                          0 if q_norm is None else _vector(dev, q_norm, "q_norm", f32, hs),
+                          0 if k_norm is None else _vector(dev, k_norm, "k_norm", f32, hs), bool(v_norm), eps)
+        rc = self._lib.g4_kv_append(self.handle, layer, rows, None if rope is None else rope.handle,
+                                    _stream(dev, stream))
+        if rc:
+            check(rc, self.ctx.handle, "g4_kv_append")
 
     def attend(self, layer: int, q, out, seqs, pos, scale: float = 1.0, window: int = 0, sinks: int = 0,
                stream=None) -> None:
@@ -281,19 +307,21 @@ class KvCache:
         of negative sequences stay, rows at negative positions get zeros."""
         import torch
 
-        f32, n = torch.float32, pos.numel()
+        dev, f32, i32, n = self.ctx.device, torch.float32, torch.int32, pos.numel()
         if not 0 <= layer < len(self.head_size):
             raise ValueError(f"layer {layer} of {len(self.head_size)}")
-        hs = self.head_size[layer]
-        if q.dim() != 2 or q.shape[1] % hs or not q.shape[1]:
+        hs, wide = self.head_size[layer], q.shape[-1]
+        heads = wide // hs
+        if not heads or heads * hs != wide:
             raise ValueError(f"q must be [rows, heads * {hs}], got {tuple(q.shape)}")
-        qp, qs = _tensor(self.ctx, q, "q", f32, n, q.shape[1])
-        op, os_ = _tensor(self.ctx, out, "out", f32, n, q.shape[1])
-        rows = KvQueriesStruct(n, q.shape[1] // hs, qp, op, qs, os_, _tensor(self.ctx, seqs, "seqs", torch.int32, n)[0],
-                               _tensor(self.ctx, pos, "pos", torch.int32, n)[0], scale, window, sinks)
+        qp, qs = _matrix(dev, q, "q", f32, n, wide)
+        op, os_ = _matrix(dev, out, "out", f32, n, wide)
+        rows = _QUERIES.pack(n, heads, qp, op, qs, os_, _vector(dev, seqs, "seqs", i32, n),
+                             _vector(dev, pos, "pos", i32, n), scale, window, sinks)
         work = _workspace(self.ctx, self._work[layer], stream)
-        check(lib().g4_kv_attend(self.handle, layer, C.byref(rows), work.data_ptr(), work.numel(),
-                                 _stream(self.ctx, stream)), self.ctx.handle, "g4_kv_attend")
+        rc = self._lib.g4_kv_attend(self.handle, layer, rows, work.data_ptr(), self._work[layer], _stream(dev, stream))
+        if rc:
+            check(rc, self.ctx.handle, "g4_kv_attend")
 
 
 def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, tokens, finished=None,
@@ -306,13 +334,17 @@ def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, t
 
     if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
+    dev, f32, i32 = ctx.device, torch.float32, torch.int32
     rows, vocab = logits.shape
-    lp, ls = _tensor(ctx, logits, "logits", torch.float32, rows, vocab)
-    sp, _ = _tensor(ctx, scores, "scores", torch.float32, rows)
-    fp = None if finished is None else _tensor(ctx, finished, "finished", torch.int32, rows)[0]
-    np_, _ = _tensor(ctx, new_scores, "new_scores", torch.float32, rows)
-    pp, _ = _tensor(ctx, parents, "parents", torch.int32, rows)
-    tp, _ = _tensor(ctx, tokens, "tokens", torch.int32, rows)
-    work = _workspace(ctx, lib().g4_beam_select_workspace(rows, vocab, beams), stream)
-    check(lib().g4_beam_select(ctx.handle, lp, ls, vocab, sp, fp, rows, beams, pad_token, np_, pp, tp,
-                               work.data_ptr(), work.numel(), _stream(ctx, stream)), ctx.handle, "g4_beam_select")
+    L = lib()
+    lp, ls = _matrix(dev, logits, "logits", f32, rows, vocab)
+    sp = _vector(dev, scores, "scores", f32, rows)
+    fp = None if finished is None else _vector(dev, finished, "finished", i32, rows)
+    np_ = _vector(dev, new_scores, "new_scores", f32, rows)
+    pp = _vector(dev, parents, "parents", i32, rows)
+    tp = _vector(dev, tokens, "tokens", i32, rows)
+    work = _workspace(ctx, L.g4_beam_select_workspace(rows, vocab, beams), stream)
+    rc = L.g4_beam_select(ctx.handle, lp, ls, vocab, sp, fp, rows, beams, pad_token, np_, pp, tp, work.data_ptr(),
+                          work.numel(), _stream(dev, stream))
+    if rc:
+        check(rc, ctx.handle, "g4_beam_select")

@@ -88,7 +88,7 @@ def test_python_layer_checks_tensors(g4):
     cache = g4.KvCache.__new__(g4.KvCache)
     cache.ctx = type("Ctx", (), {"device": 0, "handle": None})()
     cache.handle, cache.n_kv_heads, cache.head_size, cache._work = None, [1], [8], [16]
-    cache.dtype, cache._views = g4.GGMLType.F32, {}
+    cache.dtype, cache._views, cache._lib = g4.GGMLType.F32, {}, g4.lib()
     x, r = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
     for call in (lambda: cache.attend(0, x, x, r, r), lambda: cache.append(0, x, x, x, x, r, r),
                  lambda: cache.resize(r, r), lambda: cache.fork(r, r), lambda: cache.copy_pages(r, r),
@@ -98,6 +98,17 @@ def test_python_layer_checks_tensors(g4):
                  lambda: g4.beam_select(cache.ctx, r, x, 1, x, r, r)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_packed_arguments_match_the_structures():
+    """The packed forms of the Python layer have the C structures' layout."""
+    from gemma4_kt_b200 import _lib, paged
+
+    assert paged._ROWS.size == C.sizeof(_lib.KvRowsStruct) and paged._QUERIES.size == C.sizeof(_lib.KvQueriesStruct)
+    a = (3, 4, 11, 12, 13, 14, 21, 22, 23, 24, 31, 32, 33, 34, 1, 0.5)
+    assert bytes(_lib.KvRowsStruct(*a)) == paged._ROWS.pack(*a)
+    b = (3, 4, 11, 12, 21, 22, 31, 32, 0.25, 7, 8)
+    assert bytes(_lib.KvQueriesStruct(*b)) == paged._QUERIES.pack(*b)
 
 
 def test_plain_pages():
