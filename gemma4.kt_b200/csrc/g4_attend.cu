@@ -114,16 +114,37 @@ __device__ __forceinline__ RowUnits row_units(const AttendArgs& a, int seq, int 
 // what every item costs beside them (fragments of q, the warps' meeting).
 __device__ __forceinline__ int line_units(const RowUnits& r) { return r.units ? r.units + kItemUnits : 0; }
 
-// The grid's cut of the line of units, and where a CTA's run starts.
-struct Run {
-  long long w0, w1, total;  // [w0, w1) of the line's length
-  int row;                  // row of w0
-  long long row_start;      // where it begins
+// Quotient of a long dividend that is usually short: a 64-bit division costs
+// several hundred cycles, which every CTA would wait for.
+__device__ __forceinline__ long long quotient(long long x, long long d) {
+  return ((x | d) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)d) : x / d;
+}
+
+// The line's cut into runs: the first `extra` CTAs have base + 1 of it, the
+// others base (no more CTAs than length: the first ones get one each).
+struct Cut {
+  long long total, base;
+  int used, extra;
+  __device__ __forceinline__ void make(long long length, int grid) {
+    total = length;
+    used = (int)min((long long)grid, length);
+    base = used ? quotient(length, used) : 0;
+    extra = (int)(length - base * used);
+  }
+  __device__ __forceinline__ long long start(int cta) const { return cta * base + min(cta, extra); }
+  __device__ __forceinline__ int cta_of(long long x) const {
+    const long long wide = extra * (base + 1);
+    return x < wide ? (int)quotient(x, base + 1) : extra + (int)quotient(x - wide, base);
+  }
 };
 
-__device__ __forceinline__ long long run_start(long long total, int grid, int cta) {
-  return total * cta / grid;
-}
+// A CTA's run and where it starts.
+struct Run {
+  long long w0, w1;     // [w0, w1) of the line
+  int row, seq, pos;    // row of w0
+  long long row_start;  // where it begins
+  Cut cut;
+};
 
 // All threads of the CTA. Up to a row per thread one scan gives both the
 // total and the place of w0; more rows are walked a second time.
@@ -133,8 +154,11 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
   constexpr int NW = THREADS / 32;
   Run run;
   long long mine = 0, x = 0, before = 0, chunk = 0;
+  int seq = -1, pos = -1;
   auto scan = [&](int r) {  // mine: units of row r; x: of the rows up to r in this chunk; chunk: of the chunk
-    mine = r < a.n_rows ? (long long)line_units(row_units(a, a.seqs[r], a.pos[r], unit)) * items : 0;
+    seq = r < a.n_rows ? a.seqs[r] : -1;
+    pos = r < a.n_rows ? a.pos[r] : -1;
+    mine = (long long)line_units(row_units(a, seq, pos, unit)) * items;
     x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -155,20 +179,20 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
     scan(r0 + tid);
     total += chunk;
   }
-  // no more CTAs than units: the first ones get one unit each
-  const int used = (int)min((long long)grid, total);
-  run.total = total;
-  run.w0 = cta < used ? run_start(total, used, cta) : total;
-  run.w1 = cta < used ? run_start(total, used, cta + 1) : total;
-  run.row = 0;
+  run.cut.make(total, grid);
+  run.w0 = run.w1 = total;
+  run.row = run.seq = run.pos = 0;
   run.row_start = 0;
-  if (run.w0 >= run.w1) return run;
+  if (cta >= run.cut.used) return run;
+  run.w0 = run.cut.start(cta);
+  run.w1 = run.cut.start(cta + 1);
   for (int r0 = 0; r0 < a.n_rows; r0 += THREADS) {
     if (a.n_rows > THREADS) scan(r0 + tid);
     const long long start = before + x - mine;
     if (mine > 0 && start <= run.w0 && run.w0 < start + mine) {
       red[NW] = r0 + tid;
       red[NW + 1] = start;
+      red[NW + 2] = ((long long)seq << 32) | pos;
     }
     before += chunk;
     if (before > run.w0) break;
@@ -176,6 +200,8 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
   __syncthreads();
   run.row = (int)red[NW];
   run.row_start = red[NW + 1];
+  run.seq = (int)(red[NW + 2] >> 32);
+  run.pos = (int)red[NW + 2];
   return run;
 }
 
@@ -194,7 +220,7 @@ struct Walk {
     row = r.row;
     row_start = r.row_start;
     if (w >= r.w1) return;
-    ru = row_units(a, a.seqs[row], a.pos[row], unit);
+    ru = row_units(a, r.seq, r.pos, unit);
     load_row(a);
   }
   __device__ __forceinline__ bool next(const AttendArgs& a, const Run& r, int unit, int items) {
@@ -207,7 +233,7 @@ struct Walk {
         load_row(a);
         continue;
       }
-      item = (int)((w - row_start) / len);
+      item = (int)quotient(w - row_start, len);
       const int at = (int)(w - row_start - (long long)item * len), to = (int)min((long long)len, at + (r.w1 - w));
       u0 = max(0, at - kItemUnits);
       n = max(0, to - kItemUnits) - u0;
@@ -311,7 +337,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   constexpr int NW = S::kWarps, MT = S::kTiles, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
   constexpr int KG = 4;  // mma steps whose operands are read together: a 128-byte block of a 16-bit head
   extern __shared__ __align__(1024) uint8_t smraw[];
-  __shared__ long long red[NW + 3];
+  __shared__ long long red[NW + 4];
   __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock];
   __shared__ float stat[NW][kHeadBlock][2];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
@@ -690,11 +716,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 
     const bool whole = k.u0 == 0 && n == k.ru.units;
     if (!whole && k.u0 == 0) {  // goes on in other CTAs, up to the one of the item's last unit
-      const int used = (int)min((long long)gridDim.x, run.total);
-      const long long end = k.item_end();
-      int last = blockIdx.x + 1;
-      while (run_start(run.total, used, last + 1) < end) ++last;
-      pending = make_int4(row, item, first ? 0 : 1, last);
+      pending = make_int4(row, item, first ? 0 : 1, run.cut.cta_of(k.item_end() - 1));
     }
     // ---- the warps meet: common maximum, sums, O
     more = k.next(a, run, S::kUnit, items);
