@@ -85,8 +85,7 @@ struct AttendShape {
   static constexpr int kBlockBytes = kUnit * 128;         // one block of every position
   static constexpr int kRing = kStages * kStage;
   static constexpr int kQBytes = kParts * HSP * kHeadBlock * 2;
-  static constexpr int kPitch = HSP + 4;                  // floats between heads where the warps meet
-  static constexpr int kMeet = kHeadBlock * kPitch * 4;   // shares the fragments' memory
+  static constexpr int kMeet = (kHeadBlock * HSP + kWarps * kHeadBlock * 4) * 4;  // where the warps meet; shares the fragments' memory
   static constexpr int kSmem = kRing + (kQBytes > kMeet ? kQBytes : kMeet);
   static constexpr int kThreads = (kWarps + 1) * 32;
 };
@@ -202,6 +201,57 @@ __device__ Run find_run(const AttendArgs& a, int unit, int items, int cta, int g
   run.row_start = red[NW + 1];
   run.seq = (int)(red[NW + 2] >> 32);
   run.pos = (int)red[NW + 2];
+  return run;
+}
+
+// The same for up to 4 rows per lane: every warp finds the run by itself.
+__device__ __forceinline__ Run find_run_small(const AttendArgs& a, int unit, int items, int cta, int grid) {
+  const int lane = threadIdx.x & 31, per = (a.n_rows + 31) / 32;
+  int seq[4], pos[4];
+  long long len[4], mine = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = lane * per + i;
+    const bool have = i < per && r < a.n_rows;
+    seq[i] = have ? a.seqs[r] : -1;
+    pos[i] = have ? a.pos[r] : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    len[i] = (long long)line_units(row_units(a, seq[i], pos[i], unit)) * items;
+    mine += len[i];
+  }
+  long long x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  Run run;
+  run.cut.make(__shfl_sync(0xffffffffu, x, 31), grid);
+  run.w0 = run.w1 = run.cut.total;
+  run.row = run.seq = run.pos = 0;
+  run.row_start = 0;
+  if (cta >= run.cut.used) return run;
+  run.w0 = run.cut.start(cta);
+  run.w1 = run.cut.start(cta + 1);
+  long long start = x - mine;
+  bool found = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!found && len[i] > 0 && start <= run.w0 && run.w0 < start + len[i]) {
+      found = true;
+      run.row = lane * per + i;
+      run.seq = seq[i];
+      run.pos = pos[i];
+    }
+    if (!found) start += len[i];
+  }
+  const int who = __ffs(__ballot_sync(0xffffffffu, found)) - 1;
+  run.row = __shfl_sync(0xffffffffu, run.row, who);
+  run.seq = __shfl_sync(0xffffffffu, run.seq, who);
+  run.pos = __shfl_sync(0xffffffffu, run.pos, who);
+  run.row_start = __shfl_sync(0xffffffffu, start, who);
   return run;
 }
 
@@ -321,6 +371,16 @@ __device__ __forceinline__ uint32_t take_part(float& x, float& y) {
   return u;
 }
 
+// The same by truncation: three parts of 8 bits are all 24 of an fp32 number
+// exactly. For K and V on their way into the mma: integer operations, where a
+// rounding conversion of every element costs more than the products.
+__device__ __forceinline__ uint32_t cut_part(float& x, float& y) {
+  const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+  x -= __uint_as_float(u & 0xffff0000u);
+  y -= __uint_as_float(v & 0xffff0000u);
+  return __byte_perm(u, v, 0x7632);
+}
+
 // Byte offset of 16-byte chunk c of position r in a stage: 128-byte blocks of
 // all positions one after the other, chunks swizzled within a row's block.
 template <int BLOCK>
@@ -338,7 +398,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   constexpr int KG = 4;  // mma steps whose operands are read together: a 128-byte block of a 16-bit head
   extern __shared__ __align__(1024) uint8_t smraw[];
   __shared__ long long red[NW + 4];
-  __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock];
+  __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock], final_s[kHeadBlock];
   __shared__ float stat[NW][kHeadBlock][2];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ unsigned boxes[NS];  // the 16-position boxes of a stage that were loaded
@@ -355,7 +415,8 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
     fence_barrier_init();
   }
   grid_dep_launch();
-  const Run run = find_run<S::kThreads>(a, S::kUnit, items, blockIdx.x, gridDim.x, red);
+  const Run run = a.n_rows <= 128 ? find_run_small(a, S::kUnit, items, blockIdx.x, gridDim.x)
+                                  : find_run<S::kThreads>(a, S::kUnit, items, blockIdx.x, gridDim.x, red);
   __syncthreads();  // the barriers are set up (find_run may return before its last one)
   Walk k;
   k.start(a, run, S::kUnit);
@@ -583,7 +644,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 #pragma unroll
               for (int p = 0; p < 3; ++p)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ka[p][i] = take_part<false>(x[2 * i], x[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) ka[p][i] = cut_part(x[2 * i], x[2 * i + 1]);
 #pragma unroll
               for (int p = 0; p < NP; ++p) {  // products of parts i + p <= 2
                 const uint2 b = qf[(p * KS + kk) * 32 + lane];
@@ -701,7 +762,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 #pragma unroll
                 for (int p = 0; p < 3; ++p)
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) va[p][e] = take_part<false>(x[2 * e], x[2 * e + 1]);
+                  for (int e = 0; e < 4; ++e) va[p][e] = cut_part(x[2 * e], x[2 * e + 1]);
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
@@ -739,44 +800,47 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
       for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][2 * (lane & 3) + h][0]);
       f[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - M);
     }
-    // few heads leave room for several warps' sums side by side; otherwise they
-    // add up in the warps' order
-    const int side = nh <= kHeadBlock / NW ? NW : nh <= kHeadBlock / 2 ? 2 : 1, width = kHeadBlock / side;
-#pragma unroll 1
-    for (int w = 0; w < NW; w += side) {
-      if (w == warp / side * side) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int head = 2 * (lane & 3) + h;
-          if (head < nh) {
-            float* at = meet + ((warp - w) * width + head) * S::kPitch + (lane >> 2);
-#pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              at[i * 16] = (w ? at[i * 16] : 0.f) + o[i][h] * f[h];
-              at[i * 16 + 8] = (w ? at[i * 16 + 8] : 0.f) + o[i][2 + h] * f[h];
-            }
-          }
-        }
-      }
-      bar_compute<NW * 32>();
-    }
-    for (int h = warp; h < nh; h += NW) {
+    // All warps lay a range of dims of every head side by side, and all threads
+    // add them up; the fewer the heads, the wider the range.
+    const int heads = nh <= 1 ? 1 : nh <= 2 ? 2 : nh <= 4 ? 4 : 8;
+    const int width = min(HSP, HSP * kHeadBlock / (NW * heads)), shift = __ffs(width) - 1, pitch = width + 4;
+    if (tid < nh) {
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][h][0]);
+      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][tid][0]);
 #pragma unroll
-      for (int i = 0; i < NW; ++i) L += stat[i][h][0] == -INFINITY ? 0.f : exp2_approx(stat[i][h][0] - M) * stat[i][h][1];
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      float* ws = a.ws + ((long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock + h) * (hs + 2);
-      float* out = whole ? a.out + row * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs : ws + 2;
-      if (!whole && lane == 0) {
+      for (int i = 0; i < NW; ++i) L += stat[i][tid][0] == -INFINITY ? 0.f : exp2_approx(stat[i][tid][0] - M) * stat[i][tid][1];
+      final_s[tid] = L > 0.f ? 1.f / L : 0.f;
+      if (!whole) {
+        float* ws = a.ws + ((long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock + tid) * (hs + 2);
         ws[0] = M;
         ws[1] = L;
       }
-      for (int d = lane; d < hs; d += 32) {
-        float acc = meet[h * S::kPitch + d];
-        for (int i = 1; i < side; ++i) acc += meet[(i * width + h) * S::kPitch + d];
-        out[d] = whole ? acc * inv : acc;
+    }
+    float* out = whole ? a.out + row * a.out_stride + (long long)(kvh * a.group + h0) * hs
+                       : a.ws + (long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock * (hs + 2) + 2;
+    const int out_pitch = whole ? hs : hs + 2;
+#pragma unroll 1
+    for (int d0 = 0; d0 < ks * 16; d0 += width) {
+      if (d0) bar_compute<NW * 32>();  // the range before has been added up
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int head = 2 * (lane & 3) + h;
+        float* at = meet + (warp * heads + head) * pitch + (lane >> 2) - d0;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+          if (head < nh && (unsigned)(i * 16 - d0) < (unsigned)width) {
+            at[i * 16] = o[i][h] * f[h];
+            at[i * 16 + 8] = o[i][2 + h] * f[h];
+          }
+      }
+      bar_compute<NW * 32>();
+      for (int e = tid; e < nh << shift; e += NW * 32) {
+        const int h = e >> shift, d = e & (width - 1);
+        float acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) acc += meet[(w * heads + h) * pitch + d];
+        if (d0 + d < hs) out[(long long)h * out_pitch + d0 + d] = whole ? acc * final_s[h] : acc;
       }
     }
     bar_compute<NW * 32>();  // the meeting place and the statistics are free again
