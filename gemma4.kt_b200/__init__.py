@@ -16,5 +16,5 @@ from .floattensor import (  # noqa: F401
     row_shard,
 )
 from .moe import FfnMoeBlock, MoeLayer, topk  # noqa: F401
-from .model import DecoderBatch, DecoderModel, DecoderState, ModelConfig, TensorSource  # noqa: F401
+from .model import DecoderBatch, DecoderModel, DecoderState, ModelConfig, PagedBatch, TensorSource  # noqa: F401
 from .paged import KvCache, Rope, beam_select  # noqa: F401

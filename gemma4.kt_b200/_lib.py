@@ -71,6 +71,9 @@ SIGNATURES = {
     "g4_batch_step": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp]),
     "g4_batch_stream": (_vp, [_vp]),
     "g4_batch_expert_parallel": (_i, [_vp]),
+    "g4_batch_create_paged": (_i, [_vp, _i, _i, _i, _i, _i, C.POINTER(_vp)]),
+    "g4_batch_kv": (_vp, [_vp]),
+    "g4_batch_logits": (_vp, [_vp]),
     "g4_kv_create": (_i, [_vp, _vp, C.POINTER(_vp)]),
     "g4_kv_free": (_i, [_vp]),
     "g4_kv_k": (_vp, [_vp, _i]),

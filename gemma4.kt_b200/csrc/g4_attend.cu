@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
                 for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][g & 1][p], ka[g][t], b[g][p].x, b[g][p].y);
           }
         } else {
-#pragma unroll 2
+#pragma unroll 4
           for (int kk = 0; kk < ks; ++kk) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) {

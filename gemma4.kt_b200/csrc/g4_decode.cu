@@ -38,6 +38,7 @@
 #include "g4_ctx.h"
 #include "g4_gemv.cuh"
 #include "g4_internal.h"
+#include "g4_kv.h"
 
 #include <algorithm>
 #include <cmath>
@@ -1384,7 +1385,7 @@ struct g4_batch {
   unsigned* tickets = nullptr;
   float* gemm_part = nullptr;   // split-K partial sums of the batched GEMMs
   unsigned* gemm_tickets = nullptr;
-  int* h_io = nullptr;          // pinned: tokens [n_max], positions [n_max], slots [n_max]
+  int* h_io = nullptr;          // pinned: tokens, positions, slots, distinct slots and their lengths [n_max] each
   unsigned long long* h_keys = nullptr;  // pinned [n_max]
   std::map<std::tuple<int, int, int>, MmaBatchPlan> plans;
   // expert parallelism (g4_batch_expert_parallel): per layer, this rank's experts
@@ -1392,6 +1393,13 @@ struct g4_batch {
   bool ep = false;
   std::vector<g4_tensor> ep_views;  // [layer][gate_up, down]
   std::vector<g4_moe_weights> ep_moe;
+  // paged cache (g4_batch_create_paged): sequence i of the cache is slot i
+  g4_kv* kv = nullptr;
+  g4_rope *rope_full = nullptr, *rope_swa = nullptr;
+  void* att_work = nullptr;
+  size_t att_bytes = 0;
+  int *d_seq = nullptr, *d_len = nullptr;  // the step's slots and the positions they need
+  unsigned* h_flags = nullptr;             // pinned copy of the cache's status word
 
   const MmaBatchPlan* plan(int rows, int cols, int T) {
     const int ng = T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8;
@@ -1442,7 +1450,46 @@ static int batch_repack(g4_model* m) {
   return pack(m->wcls, m->cfg.vocab, dim, m->k_cls);
 }
 
-extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_batch** out) {
+// The paged cache of a batch: pages of every KV-owning layer, the rotary plans
+// of both attention types and the attention's work space.
+static int batch_paged_setup(g4_batch* b, const g4_kv_config& pages) {
+  g4_model* m = b->m;
+  g4_ctx* c = m->ctx;
+  const g4_model_config& k = m->cfg;
+  const int own = k.n_layer_kv_from_start;
+  std::vector<int> heads, sizes;
+  for (int l = 0; l < own; ++l) {
+    heads.push_back(m->n_kv[l]);
+    sizes.push_back(m->is_swa[l] ? k.head_size_swa : k.head_size_full);
+  }
+  g4_kv_config cfg = pages;
+  cfg.n_layers = own;
+  cfg.n_kv_heads = heads.data();
+  cfg.head_size = sizes.data();
+  cfg.n_seqs = b->n_max;
+  cfg.max_positions = b->max_pos;
+  if (int r = g4_kv_create(c, &cfg, &b->kv)) return r;
+  for (int swa = 0; swa < 2; ++swa) {
+    g4_rope_config r{};
+    r.head_size = r.rot_dim = swa ? k.head_size_swa : k.head_size_full;
+    r.layout = G4_ROPE_HALF;
+    r.theta = swa ? k.rope_theta_swa : k.rope_theta;
+    r.freq_factors = swa ? nullptr : m->rope_freqs.data();
+    if (int e = g4_rope_create(c, &r, swa ? &b->rope_swa : &b->rope_full)) return e;
+  }
+  for (int l = 0; l < own; ++l) b->att_bytes = std::max(b->att_bytes, g4_kv_attend_workspace(b->kv, l));
+  if (cudaMalloc(&b->att_work, b->att_bytes) != cudaSuccess ||
+      cudaMalloc(&b->d_seq, (size_t)b->n_max * 8) != cudaSuccess ||
+      cudaMallocHost(&b->h_flags, sizeof(unsigned)) != cudaSuccess) {
+    cudaGetLastError();
+    c->set_err("g4_batch_create_paged: cannot allocate the attention's work space");
+    return G4_E_NOMEM;
+  }
+  b->d_len = b->d_seq + b->n_max;
+  return 0;
+}
+
+static int batch_create(g4_model* m, int n_max, int max_positions, const g4_kv_config* pages, g4_batch** out) {
   if (!m) return G4_E_ARG;
   g4_ctx* c = m->ctx;
   const g4_model_config& k = m->cfg;
@@ -1472,9 +1519,9 @@ extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_bat
   const size_t o_sh = off; off += al(N * dim);
   const size_t o_moe = off; off += al(N * dim);
   const size_t o_log = off; off += al(N * k.vocab);
-  const size_t o_part = off; off += N * b->part_stride;
+  const size_t o_part = off; off += pages ? 0 : N * b->part_stride;
   std::vector<size_t> o_kc, o_vc;
-  for (int l = 0; l < k.n_layer_kv_from_start; ++l) {
+  for (int l = 0; l < k.n_layer_kv_from_start && !pages; ++l) {
     const int hs = m->is_swa[l] ? k.head_size_swa : k.head_size_full;
     const size_t n = al(N * max_positions * m->n_kv[l] * hs);
     o_kc.push_back(off);
@@ -1487,7 +1534,7 @@ extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_bat
   const size_t lsc_bytes = (N * (widest / 32) * 4 + 255) / 256 * 256;
   const size_t small = lim_bytes + lsc_bytes + 256 + 4 * ((N * 8 + 255) / 256 * 256) + N * k.n_heads * 4;
   if (cudaMalloc(&b->buf, off * 4) != cudaSuccess || cudaMalloc(&b->small, small) != cudaSuccess ||
-      cudaMallocHost(&b->h_io, N * 12) != cudaSuccess || cudaMallocHost(&b->h_keys, N * 8) != cudaSuccess ||
+      cudaMallocHost(&b->h_io, N * 20) != cudaSuccess || cudaMallocHost(&b->h_keys, N * 8) != cudaSuccess ||
       cudaStreamCreateWithFlags(&b->st, cudaStreamNonBlocking) != cudaSuccess) {
     cudaGetLastError();
     g4_batch_free(b);
@@ -1506,7 +1553,7 @@ extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_bat
   b->moe_out = b->buf + o_moe;
   b->logits = b->buf + o_log;
   b->part = b->buf + o_part;
-  for (int l = 0; l < k.n_layer_kv_from_start; ++l) {
+  for (int l = 0; l < k.n_layer_kv_from_start && !pages; ++l) {
     b->kc.push_back(b->buf + o_kc[l]);
     b->vc.push_back(b->buf + o_vc[l]);
   }
@@ -1560,6 +1607,12 @@ extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_bat
       return c->cuda_fail(cudaGetLastError(), "g4_batch_create: attention set-up");
     }
   }
+  if (pages) {
+    if (int r = batch_paged_setup(b, *pages)) {
+      g4_batch_free(b);
+      return r;
+    }
+  }
   if (k.n_expert > 0) {
     int r = g4_moe_layer(c, &m->L[0].moe, b->x[0], b->moe_out, n_max, nullptr, nullptr, b->st);
     if (!r) r = c->check_status(b->st);
@@ -1576,10 +1629,37 @@ extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_bat
   return 0;
 }
 
+extern "C" int g4_batch_create(g4_model* m, int n_max, int max_positions, g4_batch** out) {
+  return batch_create(m, n_max, max_positions, nullptr, out);
+}
+
+extern "C" int g4_batch_create_paged(g4_model* m, int n_max, int max_positions, int page_size, int n_pages,
+                                     int kv_type, g4_batch** out) {
+  g4_kv_config pages{};
+  pages.type = kv_type;
+  pages.page_size = page_size;
+  pages.n_pages = n_pages;
+  try {
+    return batch_create(m, n_max, max_positions, &pages, out);
+  } catch (...) {
+    m->ctx->set_err("g4_batch_create_paged: out of host memory");
+    return G4_E_NOMEM;
+  }
+}
+
+extern "C" g4_kv* g4_batch_kv(g4_batch* b) { return b ? b->kv : nullptr; }
+extern "C" const float* g4_batch_logits(g4_batch* b) { return b ? b->logits : nullptr; }
+
 extern "C" int g4_batch_free(g4_batch* b) {
   if (!b) return G4_E_ARG;
   cudaSetDevice(b->m->ctx->dev.device);
   if (b->st) cudaStreamSynchronize(b->st);
+  if (b->kv) g4_kv_free(b->kv);
+  if (b->rope_full) g4_rope_free(b->rope_full);
+  if (b->rope_swa) g4_rope_free(b->rope_swa);
+  if (b->att_work) cudaFree(b->att_work);
+  if (b->d_seq) cudaFree(b->d_seq);
+  if (b->h_flags) cudaFreeHost(b->h_flags);
   if (b->buf) cudaFree(b->buf);
   if (b->small) cudaFree(b->small);
   if (b->gemm_part) cudaFree(b->gemm_part);
@@ -1644,6 +1724,25 @@ extern "C" int g4_batch_step(g4_batch* b, const int* tokens, const int* position
   if (!ce) ce = cudaMemcpyAsync(b->d_pos, b->h_io + b->n_max, (size_t)n * 4, cudaMemcpyHostToDevice, st);
   if (!ce) ce = cudaMemcpyAsync(b->d_slot, b->h_io + 2 * b->n_max, (size_t)n * 4, cudaMemcpyHostToDevice, st);
   if (ce) return c->cuda_fail(ce, "g4_batch_step: staging");
+  if (b->kv) {  // pages for the positions of the step's slots
+    int* h_seq = b->h_io + 3 * b->n_max;
+    int* h_len = b->h_io + 4 * b->n_max;
+    int ns = 0;
+    for (int i = 0; i < n; ++i) {
+      const int sl = slots ? slots[i] : i;
+      int j = 0;
+      while (j < ns && h_seq[j] != sl) ++j;
+      if (j == ns) {
+        h_seq[ns] = sl;
+        h_len[ns++] = 0;
+      }
+      h_len[j] = std::max(h_len[j], positions[i] + 1);
+    }
+    ce = cudaMemcpyAsync(b->d_seq, h_seq, (size_t)ns * 4, cudaMemcpyHostToDevice, st);
+    if (!ce) ce = cudaMemcpyAsync(b->d_len, h_len, (size_t)ns * 4, cudaMemcpyHostToDevice, st);
+    if (ce) return c->cuda_fail(ce, "g4_batch_step: staging");
+    if (int r = kv_resize(b->kv, b->d_seq, b->d_len, ns, true, st, "g4_batch_step: pages")) return r;
+  }
   const int dim = k.dim;
   int cur = 0;
   const float* branch = nullptr;
@@ -1682,53 +1781,86 @@ extern "C" int g4_batch_step(g4_batch* b, const int* tokens, const int* position
     if (int r = batch_prologue(b, f, l == 0 ? nullptr : b->x[cur], dim, n, "batch: qkv prologue")) return r;
     if (int r = batch_gemm(b, L.k_qkv, qkv_n, dim, n, b->qkv, qkv_n, OUT_PLAIN, 0.f, nullptr, "batch: qkv")) return r;
     cur ^= 1;
-    // ---- attention, one grid row per sequence
-    AttnArgs aa{};
-    aa.qkv = b->qkv;
-    aa.hs = L.hs;
-    aa.kv_mul = k.n_heads / L.n_kv;
-    aa.kvdim = L.kvdim;
     const bool own = l < k.n_layer_kv_from_start;
-    aa.k_off = L.qdim;
-    aa.v_off = L.has_v ? L.qdim + L.kvdim : L.qdim;
-    aa.q_norm = L.q_norm;
-    aa.k_norm = L.k_norm;
-    aa.eps = k.eps;
-    aa.cr = L.swa ? m->cr_swa : m->cr_full;
-    aa.ci = L.swa ? m->ci_swa : m->ci_full;
-    aa.kc = b->kc[L.kv_src];
-    aa.vc = b->vc[L.kv_src];
-    aa.write_kv = 0;  // the step's K/V rows are written first, by batch_kv_write_kernel
-    aa.window = L.swa ? k.sliding_window : 0;
-    aa.part = b->part;
-    aa.tickets = b->tickets;
-    aa.out = b->xbk;
-    aa.ch_max = batch_ch_max(L.hs);
-    aa.status = c->status;
-    aa.pos_arr = b->d_pos;
-    aa.slot_arr = b->d_slot;
-    aa.qkv_stride = qkv_n;
-    aa.kv_stride = (long long)b->max_pos * L.kvdim;
-    aa.part_stride = (long long)b->part_stride;
-    aa.out_stride = L.qdim;
-    aa.tick_stride = k.n_heads;
-    aa.target_chunks = 8;  // the sequences give the grid its width
-    aa.heads_per_cta = aa.kv_mul;  // K/V rows staged once for the whole group
-    int nch_max = 1;
-    for (int i = 0; i < n; ++i) {
-      const int pos = positions[i];
-      const int start = aa.window > 0 ? std::max(0, pos - aa.window + 1) : 0;
-      const int len = pos - start + 1;
-      const int ch = attn_chunk(len, aa.ch_max, aa.target_chunks);
-      nch_max = std::max(nch_max, (len + ch - 1) / ch);
+    if (b->kv) {
+      // ---- attention over the pages: norms, rotary positions and the new K/V rows, then every row
+      float* q = b->qkv;
+      g4_kv_rows rows{};
+      rows.n_rows = n;
+      rows.n_heads = k.n_heads;
+      rows.q = rows.q_out = q;
+      rows.q_stride = rows.k_stride = rows.v_stride = rows.q_out_stride = qkv_n;
+      if (own) {
+        rows.k = q + L.qdim;
+        rows.v = q + (L.has_v ? L.qdim + L.kvdim : L.qdim);
+      }
+      rows.seqs = b->d_slot;
+      rows.pos = b->d_pos;
+      rows.q_norm = L.q_norm;
+      rows.k_norm = L.k_norm;
+      rows.norm_v = 1;
+      rows.eps = k.eps;
+      if (int r = g4_kv_append(b->kv, L.kv_src, &rows, L.swa ? b->rope_swa : b->rope_full, st)) return r;
+      g4_kv_queries qs{};
+      qs.n_rows = n;
+      qs.n_heads = k.n_heads;
+      qs.q = q;
+      qs.out = b->xbk;
+      qs.q_stride = qkv_n;
+      qs.out_stride = L.qdim;
+      qs.seqs = b->d_slot;
+      qs.pos = b->d_pos;
+      qs.scale = 1.f;
+      qs.window = L.swa ? k.sliding_window : 0;
+      if (int r = g4_kv_attend(b->kv, L.kv_src, &qs, b->att_work, b->att_bytes, st)) return r;
+    } else {
+      // ---- attention, one grid row per sequence
+      AttnArgs aa{};
+      aa.qkv = b->qkv;
+      aa.hs = L.hs;
+      aa.kv_mul = k.n_heads / L.n_kv;
+      aa.kvdim = L.kvdim;
+      aa.k_off = L.qdim;
+      aa.v_off = L.has_v ? L.qdim + L.kvdim : L.qdim;
+      aa.q_norm = L.q_norm;
+      aa.k_norm = L.k_norm;
+      aa.eps = k.eps;
+      aa.cr = L.swa ? m->cr_swa : m->cr_full;
+      aa.ci = L.swa ? m->ci_swa : m->ci_full;
+      aa.kc = b->kc[L.kv_src];
+      aa.vc = b->vc[L.kv_src];
+      aa.write_kv = 0;  // the step's K/V rows are written first, by batch_kv_write_kernel
+      aa.window = L.swa ? k.sliding_window : 0;
+      aa.part = b->part;
+      aa.tickets = b->tickets;
+      aa.out = b->xbk;
+      aa.ch_max = batch_ch_max(L.hs);
+      aa.status = c->status;
+      aa.pos_arr = b->d_pos;
+      aa.slot_arr = b->d_slot;
+      aa.qkv_stride = qkv_n;
+      aa.kv_stride = (long long)b->max_pos * L.kvdim;
+      aa.part_stride = (long long)b->part_stride;
+      aa.out_stride = L.qdim;
+      aa.tick_stride = k.n_heads;
+      aa.target_chunks = 8;  // the sequences give the grid its width
+      aa.heads_per_cta = aa.kv_mul;  // K/V rows staged once for the whole group
+      int nch_max = 1;
+      for (int i = 0; i < n; ++i) {
+        const int pos = positions[i];
+        const int start = aa.window > 0 ? std::max(0, pos - aa.window + 1) : 0;
+        const int len = pos - start + 1;
+        const int ch = attn_chunk(len, aa.ch_max, aa.target_chunks);
+        nch_max = std::max(nch_max, (len + ch - 1) / ch);
+      }
+      aa.chunk_stride = nch_max;
+      if (own) {
+        batch_kv_write_kernel<<<dim3(L.n_kv, n), 64, (size_t)2 * L.hs * 4, st>>>(aa);
+        if (cudaError_t e = cudaGetLastError()) return c->cuda_fail(e, "batch: K/V rows");
+      }
+      attn_fn(aa.kv_mul)<<<dim3(L.n_kv * nch_max, n), kAttnThreads, attn_smem(L.hs, aa.kv_mul, aa.ch_max), st>>>(aa);
+      if (cudaError_t e = cudaGetLastError()) return c->cuda_fail(e, "batch: attention");
     }
-    aa.chunk_stride = nch_max;
-    if (own) {
-      batch_kv_write_kernel<<<dim3(L.n_kv, n), 64, (size_t)2 * L.hs * 4, st>>>(aa);
-      if (cudaError_t e = cudaGetLastError()) return c->cuda_fail(e, "batch: K/V rows");
-    }
-    attn_fn(aa.kv_mul)<<<dim3(L.n_kv * nch_max, n), kAttnThreads, attn_smem(L.hs, aa.kv_mul, aa.ch_max), st>>>(aa);
-    if (cudaError_t e = cudaGetLastError()) return c->cuda_fail(e, "batch: attention");
     // ---- output projection
     GemvFuse plain;
     if (int r = batch_prologue(b, plain, b->xbk, L.qdim, n, "batch: o prologue")) return r;
@@ -1779,8 +1911,11 @@ extern "C" int g4_batch_step(g4_batch* b, const int* tokens, const int* position
   ce = cudaMemcpyAsync(b->h_keys, b->keys, (size_t)n * 8, cudaMemcpyDeviceToHost, st);
   if (!ce && logits_host)
     ce = cudaMemcpyAsync(logits_host, b->logits, (size_t)n * k.vocab * 4, cudaMemcpyDeviceToHost, st);
+  if (!ce && b->kv) ce = cudaMemcpyAsync(b->h_flags, b->kv->flags, sizeof(unsigned), cudaMemcpyDeviceToHost, st);
   if (ce) return c->cuda_fail(ce, "g4_batch_step: read back");
   if (int r = c->check_status(st)) return r;  // synchronises the stream
+  if (b->kv && *b->h_flags)
+    if (int r = g4_kv_check(b->kv, nullptr, st)) return r;
   if (next_tokens_host)
     for (int i = 0; i < n; ++i) next_tokens_host[i] = (int)(0xFFFFFFFFu - (uint32_t)(b->h_keys[i] & 0xFFFFFFFFull));
   return 0;

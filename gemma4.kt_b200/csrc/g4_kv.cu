@@ -104,7 +104,7 @@ __device__ __forceinline__ int page_rounds(int n_pages) { return (n_pages + kPla
 // g4_kv_resize, planning: new lengths for the entries' sequences, pages given
 // back and taken, and the list of shared last pages to copy.
 __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const int32_t* seqs, const int32_t* new_lens,
-                                                                 int n, int32_t* free_list, KvMove* moves,
+                                                                 int n, int grow_only, int32_t* free_list, KvMove* moves,
                                                                  int32_t* plan) {
   extern __shared__ int sm[];
   int* owner = sm;              // [n_seqs] first entry naming the sequence
@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
       continue;
     }
     eo[i] = old;
+    if (grow_only && en[i] < old) en[i] = old;
     shrinks |= en[i] < old;
     if (en[i] > old && old % ps != 0) {
       const int last = d.table[(size_t)s * d.max_pages + old / ps];
@@ -418,10 +419,6 @@ static size_t fork_smem(const g4_kv* kv, int n) {
   return ((size_t)kv->n_seqs + 3 * (size_t)n + (size_t)n * fork_width(n)) * 4;
 }
 
-}  // namespace g4
-
-using namespace g4;
-
 static int entries_ok(g4_kv* kv, const char* what, const void* a, const void* b, int n, int most) {
   if (n < 0 || n > most || (n > 0 && (!a || !b))) {
     kv->ctx->set_err("%s: bad arguments (%d entries, at most %d; device arrays)", what, n, most);
@@ -429,6 +426,27 @@ static int entries_ok(g4_kv* kv, const char* what, const void* a, const void* b,
   }
   return 0;
 }
+
+int kv_resize(g4_kv* kv, const int32_t* seqs, const int32_t* lens, int n, bool grow_only, cudaStream_t st,
+              const char* what) {
+  g4_ctx* c = kv->ctx;
+  if (int r = entries_ok(kv, what, seqs, lens, n, kv->n_seqs)) return r;
+  if (n == 0) return 0;
+  DeviceScope scope(c);
+  if (scope.rc) return scope.rc;
+  const KvDev d = kv_dev(kv);
+  kv_resize_kernel<<<1, kPlanThreads, resize_smem(kv, n), st>>>(d, seqs, lens, n, grow_only, kv->free_list, kv->moves,
+                                                                kv->plan);
+  cudaError_t e = cudaGetLastError();
+  if (!e)
+    e = launch_after(kv_copy_kernel, dim3(copy_grid(kv, n)), dim3(kCopyThreads), 0, st, d, kv->strips, kv->n_strips,
+                     kv->moves, kv->plan, nullptr, nullptr, 0, nullptr, 0);
+  return e ? c->cuda_fail(e, what) : 0;
+}
+
+}  // namespace g4
+
+using namespace g4;
 
 extern "C" {
 
@@ -581,20 +599,7 @@ int32_t* g4_kv_lens(const g4_kv* kv) { return kv ? kv->lens : nullptr; }
 int32_t* g4_kv_refs(const g4_kv* kv) { return kv ? kv->refs : nullptr; }
 
 int g4_kv_resize(g4_kv* kv, const int32_t* seqs, const int32_t* lens, int n, void* stream) {
-  if (!kv) return G4_E_ARG;
-  g4_ctx* c = kv->ctx;
-  if (int r = entries_ok(kv, "g4_kv_resize", seqs, lens, n, kv->n_seqs)) return r;
-  if (n == 0) return 0;
-  DeviceScope scope(c);
-  if (scope.rc) return scope.rc;
-  cudaStream_t st = (cudaStream_t)stream;
-  const KvDev d = kv_dev(kv);
-  kv_resize_kernel<<<1, kPlanThreads, resize_smem(kv, n), st>>>(d, seqs, lens, n, kv->free_list, kv->moves, kv->plan);
-  cudaError_t e = cudaGetLastError();
-  if (!e)
-    e = launch_after(kv_copy_kernel, dim3(copy_grid(kv, n)), dim3(kCopyThreads), 0, st, d, kv->strips, kv->n_strips,
-                     kv->moves, kv->plan, nullptr, nullptr, 0, nullptr, 0);
-  return e ? c->cuda_fail(e, "g4_kv_resize") : 0;
+  return kv ? kv_resize(kv, seqs, lens, n, false, (cudaStream_t)stream, "g4_kv_resize") : G4_E_ARG;
 }
 
 int g4_kv_fork(g4_kv* kv, const int32_t* src, const int32_t* dst, int n, void* stream) {
@@ -665,7 +670,7 @@ int g4_kv_check(g4_kv* kv, int* free_pages, void* stream) {
              h[0] & KV_NOT_STORED ? " an appended position has no page or lies in a shared one;" : "",
              h[0] & KV_BAD_ROW ? " a row's sequence or position is out of range or sees a position without a page;" : "",
              h[0] & KV_TIMEOUT ? " a bounded wait expired inside a kernel;" : "");
-  return h[0] == KV_NO_PAGES ? G4_E_NOMEM : G4_E_DEVICE;
+  return h[0] & KV_NO_PAGES ? G4_E_NOMEM : G4_E_DEVICE;
 }
 
 }  // extern "C"

@@ -89,6 +89,9 @@ cudaError_t launch_after(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t s
 // Set-up of the kernels of one translation unit on the current device (loads
 // them, so that a first call may be captured); cudaError_t as int.
 int kv_attend_prepare(g4_kv* kv);
+// g4_kv_resize; grow_only: a sequence that is longer than its entry asks for keeps its length.
+int kv_resize(g4_kv* kv, const int32_t* seqs, const int32_t* lens, int n, bool grow_only, cudaStream_t st,
+              const char* what);
 int rope_prepare();
 int beam_prepare();
 

@@ -399,13 +399,15 @@ int g4_kv_append(g4_kv* kv, int layer, const g4_kv_rows* rows, const g4_rope* ro
   }
   const int hs = kv->hs[layer], nkv = kv->n_kv[layer], n = rows->n_rows;
   const int nq = rows->q ? rows->n_heads : 0;
+  const bool stores = rows->k || rows->v;
   if (n < 0 || nq < 0 || nq > 4096 || (rows->q && nq < 1) ||
-      (n > 0 && (!rows->k || !rows->v || !rows->seqs || !rows->pos || !rows_ok(rows->k, rows->k_stride, nkv, hs, n) ||
-                 !rows_ok(rows->v, rows->v_stride, nkv, hs, n) ||
+      (n > 0 && (!rows->seqs || !rows->pos || (!stores && !nq) ||
+                 (stores && (!rows->k || !rows->v || !rows_ok(rows->k, rows->k_stride, nkv, hs, n) ||
+                             !rows_ok(rows->v, rows->v_stride, nkv, hs, n))) ||
                  (nq && (!rows->q_out || !rows_ok(rows->q, rows->q_stride, nq, hs, n) ||
                          !rows_ok(rows->q_out, rows->q_out_stride, nq, hs, n)))))) {
-    c->set_err("g4_kv_append: bad arguments (%d rows, %d query heads, head size %d; rows 16-byte aligned and at least "
-               "heads x head size apart)", n, nq, hs);
+    c->set_err("g4_kv_append: bad arguments (%d rows, %d query heads, head size %d; K and V together or neither; rows "
+               "16-byte aligned and at least heads x head size apart)", n, nq, hs);
     return G4_E_ARG;
   }
   if (rope && (rope->head_size != hs || rope->ctx->dev.device != c->dev.device)) {

@@ -7,6 +7,7 @@ Reference (lib/src/main/kotlin/io/github/lbenedetto/internal/):
   LlamaConfiguration          model/LlamaConfiguration.kt  -> ModelConfig
   Llama.forward               model/Llama.kt:105-408       -> DecoderState.step (one CUDA graph)
   Llama.generateTokens        model/Llama.kt:413-477       -> DecoderState.generate (greedy, GPU-resident)
+  many sequences, beam search (no counterpart)             -> DecoderBatch, PagedBatch
 """
 from __future__ import annotations
 
@@ -202,6 +203,12 @@ class DecoderModel:
     def new_batch(self, n_max: int, max_positions: int) -> "DecoderBatch":
         return DecoderBatch(self, n_max, max_positions)
 
+    def new_paged_batch(self, n_max: int, max_positions: int, page_size: int = 32, n_pages: int | None = None,
+                        dtype=GGMLType.F32) -> "PagedBatch":
+        """A batch whose slots share pages; n_pages defaults to room for every
+        slot at max_positions."""
+        return PagedBatch(self, n_max, max_positions, page_size, n_pages, dtype)
+
 
 class DecoderState:
     """LlamaState on the device (KV cache, activations, step control)."""
@@ -269,10 +276,13 @@ class DecoderBatch:
 
     def __init__(self, model: DecoderModel, n_max: int, max_positions: int):
         self.model, self.n_max, self.max_positions = model, int(n_max), int(max_positions)
+        self.handle = self._create()
+
+    def _create(self) -> C.c_void_p:
         h = C.c_void_p()
-        check(lib().g4_batch_create(model.handle, self.n_max, self.max_positions, C.byref(h)), model.ctx.handle,
-              "g4_batch_create")
-        self.handle = h
+        check(lib().g4_batch_create(self.model.handle, self.n_max, self.max_positions, C.byref(h)),
+              self.model.ctx.handle, "g4_batch_create")
+        return h
 
     def free(self) -> None:
         if getattr(self, "handle", None):
@@ -315,3 +325,87 @@ class DecoderBatch:
                                   nt.ctypes.data_as(C.c_void_p)),
               self.model.ctx.handle, "g4_batch_step")
         return lg, nt
+
+
+class PagedBatch(DecoderBatch):
+    """A DecoderBatch over a paged KV cache (g4_batch_create_paged): `cache` is
+    its KvCache, sequence i of it slot i, valid until the batch is freed.  Slots
+    may share pages: cache.fork starts one from another's history.  Calls on
+    `cache` take stream=batch.stream; a slot is freed (cache.resize to 0) before a
+    new sequence begins in it."""
+
+    def __init__(self, model: DecoderModel, n_max: int, max_positions: int, page_size: int = 32,
+                 n_pages: int | None = None, dtype=GGMLType.F32):
+        from .paged import KvCache
+
+        self.page_size, self.dtype = int(page_size), GGMLType(int(dtype))
+        self.n_pages = int(n_pages) if n_pages is not None else int(n_max) * -(-int(max_positions) // max(1, self.page_size))
+        super().__init__(model, n_max, max_positions)
+        cfg = model.cfg
+        own = range(cfg.n_layer_kv_from_start)
+        self.cache = KvCache._of_batch(model.ctx, self.handle, [cfg.n_kv_heads[l] for l in own],
+                                       [cfg.head_size(l) for l in own], self.dtype, self.page_size, self.n_pages,
+                                       self.n_max, self.max_positions)
+
+    def _create(self) -> C.c_void_p:
+        h = C.c_void_p()
+        check(lib().g4_batch_create_paged(self.model.handle, self.n_max, self.max_positions, self.page_size,
+                                          self.n_pages, int(self.dtype), C.byref(h)), self.model.ctx.handle,
+              "g4_batch_create_paged")
+        return h
+
+    def free(self) -> None:
+        if getattr(self, "cache", None) is not None:
+            self.cache.free()
+        super().free()
+
+    def beam_search(self, tokens, beams: int, n_generate: int, eos: int | None = None, pad_token: int = 0):
+        """The `beams` best continuations of a prompt by their sum of log
+        probabilities (no counterpart in Llama.generateTokens, which samples one
+        sequence): (tokens [beams, n_generate], scores [beams]), best first.  A
+        beam that has produced `eos` goes on with pad_token at its score.  Uses
+        slots 0..beams - 1, which are free before and after; selection, reordering
+        and page bookkeeping stay on the device, a step's tokens go through the host."""
+        import torch
+
+        from .paged import _DeviceArray, _Owner, beam_select
+
+        prompt = np.ascontiguousarray(tokens, np.int32).reshape(-1)
+        if not 1 <= beams <= self.n_max or not prompt.size or n_generate < 1:
+            raise ValueError(f"{beams} beams of {self.n_max} slots, {prompt.size} prompt tokens, {n_generate} generated")
+        if prompt.size + n_generate - 1 > self.max_positions:
+            raise ValueError(f"{prompt.size} + {n_generate} tokens exceed {self.max_positions} positions")
+        ctx, vocab = self.model.ctx, self.model.cfg.vocab
+        dev = torch.device("cuda", ctx.device)
+        with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=dev)):
+            last = torch.as_tensor(_DeviceArray(_Owner(None, None), lib().g4_batch_logits(self.handle),
+                                                (self.n_max, vocab), "<f4"), device=dev)
+            rows = torch.arange(beams, dtype=torch.int32, device=dev)
+            scores = torch.full((beams,), -torch.inf, device=dev)
+            scores[0] = 0.0  # one history until the first selection
+            done = torch.zeros(beams, dtype=torch.int32, device=dev)
+            parents, chosen = torch.empty_like(rows), torch.empty_like(rows)
+            try:
+                for at in range(0, prompt.size, self.n_max):
+                    part = prompt[at:at + self.n_max]
+                    self.step(part, np.arange(at, at + part.size), want_logits=False, slots=np.zeros(part.size, np.int32))
+                logits = torch.zeros((beams, vocab), device=dev)
+                logits[0] = last[part.size - 1]
+                history = np.empty((beams, n_generate), np.int32)
+                for i in range(n_generate):
+                    beam_select(ctx, logits, scores, beams, scores, parents, chosen, finished=done, pad_token=pad_token)
+                    self.cache.fork(parents, rows)
+                    par, tok = parents.clamp(min=0), torch.where(parents < 0, pad_token, chosen)
+                    done = done[par.long()] | (parents < 0).int()
+                    if eos is not None:
+                        done |= (tok == eos).int()
+                    par, tok = par.cpu().numpy(), tok.cpu().numpy()
+                    history = history[par]
+                    history[:, i] = tok
+                    if i + 1 < n_generate:
+                        self.step(tok, np.full(beams, prompt.size + i), want_logits=False)
+                        logits = last[:beams]
+                return history, scores.cpu().numpy()
+            finally:
+                self.cache.resize(rows, torch.zeros_like(rows))
+                torch.cuda.current_stream().synchronize()

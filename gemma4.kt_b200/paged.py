@@ -169,12 +169,22 @@ class KvCache:
         if rc == -1:
             raise ValueError(ctx.last_error())
         check(rc, ctx.handle, "g4_kv_create")
-        self.ctx, self.handle = ctx, h
-        self._owner = _Owner(h, lib().g4_kv_free)
+        self._describe(ctx, h, _Owner(h, lib().g4_kv_free), heads, sizes, dtype, page_size, n_pages, n_seqs,
+                       max_positions)
+
+    @staticmethod
+    def _of_batch(ctx: Context, batch_handle, *description) -> "KvCache":
+        """The cache of a paged batch, which owns it: it and its views end with the batch."""
+        cache = KvCache.__new__(KvCache)
+        cache._describe(ctx, C.c_void_p(lib().g4_batch_kv(batch_handle)), _Owner(None, None), *description)
+        return cache
+
+    def _describe(self, ctx, handle, owner, heads, sizes, dtype, page_size, n_pages, n_seqs, max_positions) -> None:
+        self.ctx, self.handle, self._owner = ctx, handle, owner
         self.n_kv_heads, self.head_size = [int(x) for x in heads], [int(x) for x in sizes]
         self.dtype, self.page_size, self.n_pages, self.n_seqs = GGMLType(int(dtype)), page_size, n_pages, n_seqs
         self.max_positions, self.max_pages = max_positions, -(-max_positions // page_size)
-        self._work = [lib().g4_kv_attend_workspace(h, l) for l in range(heads.size)]
+        self._work = [lib().g4_kv_attend_workspace(handle, l) for l in range(len(self.head_size))]
         self._views = {}
         self._lib = lib()
 
@@ -272,7 +282,8 @@ class KvCache:
                v_norm: bool = False, eps: float = 1e-6, stream=None) -> None:
         """Row i is position pos[i] of sequence seqs[i]: its K and V rows, normed
         and rotated, go into their page, its normed and rotated queries to q_out
-        (which may be q; q and q_out None: K and V alone).  fp32 rows
+        (which may be q; q and q_out None: K and V alone; k and v None: queries
+        alone, for a layer that reads another layer's cache).  fp32 rows
         [rows, heads * head_size] with any row stride."""
         import torch
 
@@ -280,9 +291,10 @@ class KvCache:
         if not 0 <= layer < len(self.head_size):
             raise ValueError(f"layer {layer} of {len(self.head_size)}")
         hs, width = self.head_size[layer], self.n_kv_heads[layer] * self.head_size[layer]
-        kp, ks = _matrix(dev, k, "k", f32, n, width)
-        vp, vs = _matrix(dev, v, "v", f32, n, width)
-        heads = qp = qs = op = os_ = 0
+        heads = qp = qs = op = os_ = kp = ks = vp = vs = 0
+        if k is not None or v is not None:
+            kp, ks = _matrix(dev, k, "k", f32, n, width)
+            vp, vs = _matrix(dev, v, "v", f32, n, width)
         if q is not None:
             wide = q.shape[-1]
             heads = wide // hs

@@ -314,6 +314,22 @@ int g4_batch_step(g4_batch *batch, const int *tokens, const int *positions, cons
                   float *logits_host, int *next_tokens_host);
 /* The batch's cudaStream_t. */
 void *g4_batch_stream(g4_batch *batch);
+/* A batch whose KV cache lies in pages that its slots may share (g4_kv, below):
+ * n_pages pages of page_size positions of every KV-owning layer, rounded to
+ * kv_type (G4_TYPE_F32, F16 or BF16), instead of n_max * max_positions fp32
+ * positions.  g4_batch_step gives a slot pages for its new positions by itself
+ * (G4_E_NOMEM when there are none); slots are forked, freed and compacted with
+ * the g4_kv calls on g4_batch_kv (sequence i = slot i) on the batch's stream.
+ * A slot is freed (resized to 0) before a new sequence begins in it.  Head sizes
+ * 8..512 in steps of 8. */
+typedef struct g4_kv g4_kv;
+int g4_batch_create_paged(g4_model *model, int n_max, int max_positions, int page_size, int n_pages, int kv_type,
+                          g4_batch **out);
+/* The batch's cache, owned by it (NULL: not paged). */
+g4_kv *g4_batch_kv(g4_batch *batch);
+/* Device logits [n][vocab] of the last step (after softcapping), overwritten by
+ * the next: for g4_beam_select on the batch's stream. */
+const float *g4_batch_logits(g4_batch *batch);
 /* Expert parallelism for a batch (no counterpart in the reference, which runs
  * in one process): after g4_dist_init on W >= 2 ranks, rank r computes experts
  * [r*E/W, (r+1)*E/W) of every MoE layer for all ranks' tokens (the layer runs
@@ -343,7 +359,6 @@ int g4_batch_expert_parallel(g4_batch *batch);
  * that change one cache (resize, fork, compact, copy_pages, append) must be
  * ordered on the GPU, among each other and with the calls that read it;
  * g4_kv_attend calls may overlap if each has its own work space. */
-typedef struct g4_kv g4_kv;
 typedef struct {
   int n_layers;
   const int *n_kv_heads;  /* [n_layers] 1..256 */
@@ -385,8 +400,9 @@ int g4_kv_compact(g4_kv *kv, void *stream);
  * Destinations distinct and no sources; pairs with a negative number are
  * padding. n <= n_pages. */
 int g4_kv_copy_pages(g4_kv *kv, const int32_t *src_dev, const int32_t *dst_dev, int n, void *stream);
-/* Waits for `stream`; G4_E_NOMEM after a resize that lacked pages, G4_E_DEVICE
- * after skipped entries or rows, with the message; the record is cleared.
+/* Waits for `stream`; G4_E_NOMEM after a resize that lacked pages, otherwise
+ * G4_E_DEVICE after skipped entries or rows, with the message; the record is
+ * cleared.
  * free_pages may be NULL.  Not during a capture (G4_E_ARG). */
 int g4_kv_check(g4_kv *kv, int *free_pages, void *stream);
 
@@ -429,7 +445,8 @@ int g4_rope_apply(const g4_rope *rope, const float *x_dev, int64_t x_stride, flo
  * projection; rows 16-byte aligned. */
 typedef struct {
   int n_rows;
-  int n_heads;                    /* query heads; with q == NULL only K and V are stored */
+  int n_heads;                    /* query heads; q NULL: only K and V are stored; k and v NULL: only queries (a layer
+                                     that reads another layer's cache) */
   const float *q, *k, *v;         /* device, [n_rows][heads * head_size] */
   float *q_out;                   /* may be q */
   int64_t q_stride, k_stride, v_stride, q_out_stride;
