@@ -596,13 +596,18 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
       uint32_t pf[MT][NP][2];
       bool partial = false;
       {
-        // sums by part and by even and odd step: enough independent chains to
-        // cover an mma's latency
-        float s[MT][2][NP][4];
+        // The tensor core cuts its sums off instead of rounding them, so the first
+        // parts' products, which carry the score, go into fresh sums every few steps
+        // and are added in fp32; the others' (2^-8 and less) stay in one chain each.
+        float main[MT][4], s[MT][NP][4];
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-          for (int p = 0; p < 2 * NP; ++p) s[t][p / NP][p % NP][0] = s[t][p / NP][p % NP][1] = s[t][p / NP][p % NP][2] = s[t][p / NP][p % NP][3] = 0.f;
+          for (int i = 0; i < 4; ++i) {
+            main[t][i] = 0.f;
+#pragma unroll
+            for (int p = 0; p < NP; ++p) s[t][p][i] = 0.f;
+          }
         const uint32_t kt = ring + stage * S::kStage;
         const uint8_t* kg = smraw + stage * S::kStage;
         if (TYPE != F32) {
@@ -619,12 +624,24 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
               for (int t = 0; t < MT; ++t)
                 ldsm4(ka[g][t], kt + chunk_at<BLK>((warp * MT + t) * kTile + (lane & 15), 2 * (k0 + g) + (lane >> 4)));
             }
+            float fresh[2][MT][4];
 #pragma unroll
-            for (int g = 0; g < KG; ++g)
+            for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int p = 0; p < NP; ++p)
+              for (int i = 0; i < 4; ++i) fresh[0][t][i] = fresh[1][t][i] = 0.f;
 #pragma unroll
-                for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][g & 1][p], ka[g][t], b[g][p].x, b[g][p].y);
+            for (int g = 0; g < KG; ++g) {
+#pragma unroll
+              for (int t = 0; t < MT; ++t) mma16816<HALF>(fresh[g & 1][t], ka[g][t], b[g][0].x, b[g][0].y);
+#pragma unroll
+              for (int p = 1; p < NP; ++p)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][p], ka[g][t], b[g][p].x, b[g][p].y);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) main[t][i] += fresh[0][t][i] + fresh[1][t][i];
           }
         } else {
 #pragma unroll 4
@@ -645,12 +662,15 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
               for (int p = 0; p < 3; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) ka[p][i] = cut_part(x[2 * i], x[2 * i + 1]);
+              float fresh[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int p = 0; p < NP; ++p) {  // products of parts i + p <= 2
                 const uint2 b = qf[(p * KS + kk) * 32 + lane];
 #pragma unroll
-                for (int i = 0; i < 3 - p; ++i) mma16816<false>(s[t][p & 1][i], ka[i], b.x, b.y);
+                for (int i = 0; i < 3 - p; ++i) mma16816<false>(i + p == 0 ? fresh : s[t][i], ka[i], b.x, b.y);
               }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) main[t][i] += fresh[i];
             }
           }
         }
@@ -664,9 +684,10 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
           partial |= !whole;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = s[t][0][NP - 1][i] + s[t][1][NP - 1][i];
+            float v = s[t][NP - 1][i];
 #pragma unroll
-            for (int p = NP - 2; p >= 0; --p) v += s[t][0][p][i] + s[t][1][p][i];
+            for (int p = NP - 2; p >= 0; --p) v += s[t][p][i];
+            v += main[t][i];
             const bool vis = whole || (have && k.seen(tt + (lane >> 2) + (i >> 1) * 8, a.sinks));
             x[t][i] = vis ? v * sc[i & 1] : -INFINITY;
           }
@@ -726,10 +747,14 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
+        // (a tile's sums are fresh, too, and added to O in fp32)
         if (TYPE != F32) {
 #pragma unroll
           for (int i = 0; i < KS; i += KG) {
             if (i < ks) {
+              float fresh[KG][4];
+#pragma unroll
+              for (int g = 0; g < KG; ++g) fresh[g][0] = fresh[g][1] = fresh[g][2] = fresh[g][3] = 0.f;
 #pragma unroll
               for (int t = 0; t < MT; ++t) {
                 uint32_t va[KG][4];
@@ -740,14 +765,19 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-                  for (int g = 0; g < KG; ++g) mma16816<HALF>(o[i + g], va[g], pf[t][p][0], pf[t][p][1]);
+                  for (int g = 0; g < KG; ++g) mma16816<HALF>(fresh[g], va[g], pf[t][p][0], pf[t][p][1]);
               }
+#pragma unroll
+              for (int g = 0; g < KG; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i + g][e] += fresh[g][e];
             }
           }
         } else {
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
             if (i < ks) {
+              float fresh[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
               for (int t = 0; t < MT; ++t) {
                 // V[pos 2 (lane % 4) + {0, 1} (+ 8)][dim lane / 4 (+ 8)]: registers (dim), (dim + 8), then pos + 8
@@ -766,8 +796,10 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-                  for (int e = 2 - p; e >= 0; --e) mma16816<false>(o[i], va[e], pf[t][p][0], pf[t][p][1]);
+                  for (int e = 2 - p; e >= 0; --e) mma16816<false>(fresh, va[e], pf[t][p][0], pf[t][p][1]);
               }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[i][e] += fresh[e];
             }
           }
         }
