@@ -481,6 +481,7 @@ int g4_kv_create(g4_ctx* c, const g4_kv_config* cfg, g4_kv** out) {
   g4_kv* kv = new (std::nothrow) g4_kv();
   if (!kv) return G4_E_NOMEM;
   kv->ctx = c;
+  kv->device = c->dev.device;
   std::vector<KvStrip> strips;
   uint64_t bytes = 0;
   try {
@@ -580,7 +581,7 @@ int g4_kv_create(g4_ctx* c, const g4_kv_config* cfg, g4_kv** out) {
 int g4_kv_free(g4_kv* kv) {
   if (!kv) return G4_E_ARG;
   {
-    DeviceScope scope(kv->ctx);
+    DeviceScope scope(kv->device);
     if (kv->pool) cudaFree(kv->pool);
     if (kv->meta) cudaFree(kv->meta);
   }

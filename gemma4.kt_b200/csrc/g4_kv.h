@@ -36,6 +36,7 @@ struct KvMove {
 
 struct g4_kv {
   g4_ctx* ctx = nullptr;
+  int device = 0;
   int n_layers = 0, type = 0, elem = 0, page_size = 0, page_shift = 0, n_pages = 0, n_seqs = 0, max_positions = 0;
   int max_pages = 0;  // pages of one sequence (the table's width)
   int n_strips = 0;
@@ -59,10 +60,15 @@ namespace g4 {
 struct DeviceScope {
   int prev = -1, rc = 0;
   explicit DeviceScope(g4_ctx* c) {
+    if (const cudaError_t e = enter(c->dev.device)) rc = c->cuda_fail(e, "cudaSetDevice");
+  }
+  // For handles that are freed after their context.
+  explicit DeviceScope(int device) { rc = enter(device); }
+  cudaError_t enter(int device) {
     cudaError_t e = cudaGetDevice(&prev);
-    if (e == cudaSuccess && prev != c->dev.device) e = cudaSetDevice(c->dev.device);
+    if (e == cudaSuccess && prev != device) e = cudaSetDevice(device);
     else prev = -1;
-    if (e != cudaSuccess) rc = c->cuda_fail(e, "cudaSetDevice");
+    return e;
   }
   ~DeviceScope() {
     if (prev >= 0) cudaSetDevice(prev);

@@ -25,6 +25,7 @@
 
 struct g4_rope {
   g4_ctx* ctx = nullptr;
+  int device = 0;
   int head_size = 0, rot = 0, interleaved = 0;
   float factor = 1.f;
   double* turns = nullptr;  // [rot / 2] turns per position
@@ -325,6 +326,7 @@ int g4_rope_create(g4_ctx* c, const g4_rope_config* cfg, g4_rope** out) {
   g4_rope* r = new (std::nothrow) g4_rope();
   if (!r) return G4_E_NOMEM;
   r->ctx = c;
+  r->device = c->dev.device;
   r->head_size = cfg->head_size;
   r->rot = rot;
   r->interleaved = cfg->layout == G4_ROPE_INTERLEAVED;
@@ -352,7 +354,7 @@ int g4_rope_create(g4_ctx* c, const g4_rope_config* cfg, g4_rope** out) {
 int g4_rope_free(g4_rope* r) {
   if (!r) return G4_E_ARG;
   {
-    DeviceScope scope(r->ctx);
+    DeviceScope scope(r->device);
     if (r->turns) cudaFree(r->turns);
   }
   delete r;
@@ -410,9 +412,9 @@ int g4_kv_append(g4_kv* kv, int layer, const g4_kv_rows* rows, const g4_rope* ro
                "16-byte aligned and at least heads x head size apart)", n, nq, hs);
     return G4_E_ARG;
   }
-  if (rope && (rope->head_size != hs || rope->ctx->dev.device != c->dev.device)) {
+  if (rope && (rope->head_size != hs || rope->device != c->dev.device)) {
     c->set_err("g4_kv_append: the rotary plan is for head size %d on device %d, the layer has %d on %d",
-               rope->head_size, rope->ctx->dev.device, hs, c->dev.device);
+               rope->head_size, rope->device, hs, c->dev.device);
     return G4_E_ARG;
   }
   if ((reinterpret_cast<uintptr_t>(rows->q_norm) | reinterpret_cast<uintptr_t>(rows->k_norm)) & 7) {

@@ -457,7 +457,7 @@ typedef struct {
 } g4_kv_rows;
 /* Llama.kt:157-195 for the rows: q_out = rotated, normed q; the normed, rotated
  * K row and the (normed) V row go into their page, rounded to the cache's type
- * (nearest).  rope NULL: no rotation.  A row with seqs[i] < 0 is padding and
+ * (nearest; beyond f16's range to infinity).  rope NULL: no rotation.  A row with seqs[i] < 0 is padding and
  * left as it was; (sequence, position) pairs distinct.  A position without a
  * page, or in a page that sequences share, is not stored (g4_kv_check). */
 int g4_kv_append(g4_kv *kv, int layer, const g4_kv_rows *rows, const g4_rope *rope, void *stream);
@@ -466,7 +466,7 @@ typedef struct {
   int n_rows;
   int n_heads;                /* a multiple of the layer's KV heads; query head h reads KV head h / (n_heads / n_kv) */
   const float *q;             /* device [n_rows][n_heads * head_size] */
-  float *out;
+  float *out;                 /* may be q */
   int64_t q_stride, out_stride;
   const int32_t *seqs, *pos;  /* device [n_rows] */
   float scale;                /* of the scores (1 in Llama.kt:204-208) */
@@ -490,7 +490,8 @@ int g4_kv_attend(g4_kv *kv, int layer, const g4_kv_queries *rows, void *work, si
  * Ties go to the lower beam, then the lower token.  parents are row numbers
  * (g4_kv_fork's src).  finished_dev (int32, NULL: none): a finished row has one
  * continuation, pad_token at its own score.  Logits of -inf (masked tokens) and
- * NaN are never chosen; where too few remain: score -inf, parent and token -1.
+ * NaN are never chosen (a row with a logit of +inf has no continuation); where
+ * too few remain: score -inf, parent and token -1.
  * new_scores may be scores.  beams <= 32; work as for g4_kv_attend. */
 size_t g4_beam_select_workspace(int n_rows, int vocab, int beams);
 int g4_beam_select(g4_ctx *ctx, const float *logits_dev, int64_t stride, int vocab, const float *scores_dev,

@@ -400,6 +400,21 @@ def test_attend_empty_and_padding_rows(g4, ctx):
     attend_case(g4, ctx, "f32", 64, 1, 4, 16, [(0, -1)] * 3)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attend_in_place(g4, ctx, kind):
+    cache = new_cache(g4, ctx, kind, (2,), (64,), 16, 700, 9, 1200)
+    cache.resize(i32(range(9)), i32([1200] * 9))
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for p in (cache.k(0), cache.v(0)):
+        p.copy_(torch.randn(p.shape, generator=g, device="cuda"))
+    q = torch.randn(9, 20 * 64, generator=g, device="cuda")
+    pos = i32([0, 1199, 5, 700, 64, -1, 31, 1198, 300])
+    out = torch.empty_like(q)
+    cache.attend(0, q, out, i32(range(9)), pos, scale=0.1)
+    cache.attend(0, q, q, i32(range(9)), pos, scale=0.1)
+    assert torch.equal(q, out)
+
+
 def test_attend_rows_of_one_sequence(g4, ctx):
     """A prompt chunk: many rows of few sequences, each up to its own position."""
     rows = [(s, p) for s in range(3) for p in range(100, 200)]
@@ -524,6 +539,19 @@ def test_beam_ordered_logits(g4, ctx, beams):
     rows = np.stack([up, up[::-1], np.zeros(vocab, np.float32), saw, np.round(up), np.where(up > 9.9, up, -np.inf)])
     rows = np.repeat(rows, beams, axis=0).astype(np.float32)
     check_beams(g4, ctx, rows, np.tile(-np.arange(beams) * 0.125, 6).astype(np.float32), beams)
+
+
+def test_beam_infinite_logits(g4, ctx):
+    """A row with +inf has no continuation; its group's others go on."""
+    rng = np.random.default_rng(3)
+    logits = rng.standard_normal((4, 3000)).astype(np.float32)
+    logits[1, 1500] = np.inf
+    scores = np.zeros(4, np.float32)
+    got = select(g4, ctx, torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda(), 4)
+    masked = logits.copy()
+    masked[1] = -np.inf
+    want = ref.beam(masked, scores, 4)
+    assert np.array_equal(host(got[1]), want[1]) and np.array_equal(host(got[2]), want[2])
 
 
 def test_beam_strided_and_in_place(g4, ctx):
@@ -675,6 +703,19 @@ def test_calls_on_other_streams(g4, ctx):
     torch.cuda.synchronize()
     for a, b in zip(want, got):
         assert torch.equal(a, b)
+
+
+def test_handles_outlive_their_context(g4):
+    """Views keep the pages alive; the context may go first."""
+    c = g4.Context(0)
+    cache = new_cache(g4, c, kv=(1,), hs=(16,), pages=4)
+    rope = g4.Rope(c, 16)
+    view = cache.k(0)
+    view.fill_(2.0)
+    del cache
+    c.close()
+    assert float(view.sum()) == 2.0 * view.numel()
+    del view, rope
 
 
 # ------------------------------------------------------------------ refusals
