@@ -48,6 +48,8 @@ constexpr int kHeadBlock = 8;  // query heads per item: the mma's columns
 constexpr int kTile = 16;      // positions per warp and step: the mma's rows
 constexpr int kJoinThreads = 256;
 constexpr int kItemUnits = 1;
+constexpr int kMaxGrid = 512;  // CTAs (a B200 takes 296)
+static_assert(kKvMaxHeadSize <= 2 * kJoinThreads, "two dims per thread of the join");
 
 struct AttendArgs {
   const float* q;
@@ -63,7 +65,7 @@ struct AttendArgs {
   float scale_log2;         // scale * log2(e): scores in powers of two
   int window, sinks;
   float* ws;                // [grid][2][kHeadBlock][hs + 2] partials: max, sum, O
-  int4* joins;              // [grid] the item a CTA begins and others go on with (x < 0: none)
+  int4* joins;              // [grid] the item that a CTA goes on with: row (-1: none), item, first CTA and its slot, last CTA
 };
 
 // Shape of one instantiation: element type, padded head size, warps that
@@ -531,9 +533,9 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
     }
   };
   bool first = true, more = k.next(a, run, S::kUnit, items);
+  if (tid == 0 && (!more || k.u0 == 0)) a.joins[blockIdx.x].x = -1;
   constexpr bool kAhead = QL <= 8;  // room in registers to read q during the meeting before
   if (kAhead && more) load_q();
-  int4 pending = make_int4(-1, 0, 0, 0);  // the item that goes on in the next CTA
   while (more) {
     const int row = k.row, item = k.item, n = k.n;
     const int kvh = item / a.blocks, h0 = (item - kvh * a.blocks) * kHeadBlock, nh = min(kHeadBlock, a.group - h0);
@@ -808,8 +810,11 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
     }
 
     const bool whole = k.u0 == 0 && n == k.ru.units;
-    if (!whole && k.u0 == 0) {  // goes on in other CTAs, up to the one of the item's last unit
-      pending = make_int4(row, item, first ? 0 : 1, run.cut.cta_of(k.item_end() - 1));
+    if (k.u0 > 0 && tid == 0) {  // begun by another CTA: where its parts are, for the join
+      const long long end = k.item_end(), begin = end - line_units(k.ru);
+      const int from = run.cut.cta_of(begin + kItemUnits);
+      const int slot = run.cut.start(from) < begin;  // the first of its CTA's parts, or its last
+      a.joins[blockIdx.x] = make_int4(row, item, from * 2 + slot, run.cut.cta_of(end - 1));
     }
     // ---- the warps meet: common maximum, sums, O
     more = k.next(a, run, S::kUnit, items);
@@ -878,63 +883,70 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
     bar_compute<NW * 32>();  // the meeting place and the statistics are free again
     first = false;
   }
-  if (tid == 0) a.joins[blockIdx.x] = pending;
 }
 
-// Joins the partials of items that span CTAs: block (c, h) takes head h of the
-// item that starts in CTA c and does not end there.
+// Joins the partials of items that span CTAs. Block (c, h) belongs to the item
+// that CTA c goes on with: its CTAs but the first share the dims of head h, so
+// the longer the item, the more blocks work on it.
 __global__ void __launch_bounds__(kJoinThreads) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
-  __shared__ float wsum[kJoinThreads / 32];
-  __shared__ float acc_s[kJoinThreads / 32][kKvMaxHeadSize];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, c = blockIdx.x, h = blockIdx.y;
+  __shared__ float red[kJoinThreads / 32];
+  __shared__ float weight[kMaxGrid], sum[kMaxGrid];
+  __shared__ __align__(8) float acc_s[2 * kJoinThreads];  // [group][dims]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, h = blockIdx.y;
   constexpr int NW = kJoinThreads / 32;
   grid_dep_wait();
-  const int4 j = __ldcg(a.joins + c);  // row, item, slot in c, last CTA
+  const int4 j = __ldcg(a.joins + blockIdx.x);
   if (j.x < 0) return;
-  const int kvh = j.y / a.blocks, h0 = (j.y - kvh * a.blocks) * kHeadBlock, last = j.w;
+  const int kvh = j.y / a.blocks, h0 = (j.y - kvh * a.blocks) * kHeadBlock, c = j.z >> 1, slot = j.z & 1;
   if (h >= min(kHeadBlock, a.group - h0)) return;
+  const int n = j.w - c + 1;  // partials, in CTAs c..c + n - 1
+  const int share = (hs / 2 + n - 2) / (n - 1), d0 = 2 * share * ((int)blockIdx.x - c - 1);
+  const int per = min(share, (hs - d0) / 2);  // pairs of dims
+  if (per <= 0) return;
   auto partial = [&](int i) {  // of CTA i
-    return a.ws + ((long long)(i * 2 + (i == c ? j.z : 0)) * kHeadBlock + h) * (hs + 2);
+    return a.ws + ((long long)(i * 2 + (i == c ? slot : 0)) * kHeadBlock + h) * (hs + 2);
   };
+  // every partial's weight: 2^(its maximum - the common one)
   float M = -INFINITY;
-  for (int i = c + lane; i <= last; i += 32) M = fmaxf(M, __ldcg(partial(i)));
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(partial(c + i)));
+    weight[i] = ml.x;
+    sum[i] = ml.y;
+    M = fmaxf(M, ml.x);
+  }
 #pragma unroll
   for (int b = 16; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
+  if (lane == 0) red[warp] = M;
+  __syncthreads();
+  M = red[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) M = fmaxf(M, red[i]);
   if (M == -INFINITY) M = 0.f;
-  // a warp takes every NW-th partial; lanes pairs of dims
-  float2 acc[kKvMaxHeadSize / 64];
-  float L = 0.f;
-#pragma unroll
-  for (int u = 0; u < kKvMaxHeadSize / 64; ++u) acc[u] = make_float2(0.f, 0.f);
-  for (int i = c + warp; i <= last; i += NW) {
-    const float* p = partial(i);
-    const float f = exp2_approx(__ldcg(p) - M);
-    L = fmaf(f, __ldcg(p + 1), L);
-#pragma unroll
-    for (int u = 0; u < kKvMaxHeadSize / 64; ++u) {
-      const int d = 2 * (lane + 32 * u);
-      if (d < hs) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(p + 2 + d));
-        acc[u].x = fmaf(f, v.x, acc[u].x);
-        acc[u].y = fmaf(f, v.y, acc[u].y);
-      }
-    }
-  }
-  if (lane == 0) wsum[warp] = L;
-#pragma unroll
-  for (int u = 0; u < kKvMaxHeadSize / 64; ++u) {
-    const int d = 2 * (lane + 32 * u);
-    if (d < hs) *reinterpret_cast<float2*>(&acc_s[warp][d]) = acc[u];
+  for (int i = tid; i < n; i += kJoinThreads) {  // (the thread's own entries)
+    weight[i] = exp2_approx(weight[i] - M);
+    sum[i] *= weight[i];
   }
   __syncthreads();
-  for (int d = tid; d < hs; d += kJoinThreads) {
-    float s = 0.f, t = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      s += acc_s[i][d];
-      t += wsum[i];
+  // threads own two dims each; groups of them take every groups-th partial
+  const int groups = kJoinThreads / per, g = tid / per, d = 2 * (tid - g * per);
+  if (g < groups) {
+    float2 acc = make_float2(0.f, 0.f);
+#pragma unroll 8
+    for (int i = g; i < n; i += groups) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(partial(c + i) + 2 + d0 + d));
+      acc.x = fmaf(weight[i], v.x, acc.x);
+      acc.y = fmaf(weight[i], v.y, acc.y);
     }
-    a.out[j.x * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d] = t > 0.f ? s / t : 0.f;
+    *reinterpret_cast<float2*>(acc_s + g * 2 * per + d) = acc;
+  }
+  float L = 0.f;
+  for (int i = lane; i < n; i += 32) L += sum[i];
+  L = warp_sum(L);
+  __syncthreads();
+  for (int e = tid; e < 2 * per; e += kJoinThreads) {
+    float s = 0.f;
+    for (int i = 0; i < min(groups, n); ++i) s += acc_s[i * 2 * per + e];
+    a.out[j.x * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d0 + e] = L > 0.f ? s / L : 0.f;
   }
 }
 
@@ -973,6 +985,11 @@ static bool make_map(PFN_cuTensorMapEncodeTiled_v12000 encode, CUtensorMap* map,
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+static int attend_grid(const g4_ctx* c, const AttendPlan& p) {
+  const int full = c->dev.sms * p.ctas;
+  return full < kMaxGrid ? full : kMaxGrid;
+}
+
 int kv_attend_prepare(g4_kv* kv) {
   void* entry = nullptr;
   cudaDriverEntryPointQueryResult q{};
@@ -1001,7 +1018,7 @@ extern "C" {
 size_t g4_kv_attend_workspace(const g4_kv* kv, int layer) {
   if (!kv || layer < 0 || layer >= kv->n_layers) return 0;
   const AttendPlan p = attend_plan(kv->type, kv->hs[layer]);
-  const size_t grid = (size_t)kv->ctx->dev.sms * p.ctas;
+  const size_t grid = attend_grid(kv->ctx, p);
   return grid * (sizeof(int4) + 2 * kHeadBlock * (kv->hs[layer] + 2) * sizeof(float));
 }
 
@@ -1054,7 +1071,7 @@ int g4_kv_attend(g4_kv* kv, int layer, const g4_kv_queries* rows, void* work, si
   a.window = rows->window;
   a.sinks = rows->window > 0 ? rows->sinks : 0;
   const AttendPlan p = attend_plan(kv->type, hs);
-  const int grid = c->dev.sms * p.ctas;
+  const int grid = attend_grid(c, p);
   a.joins = static_cast<int4*>(work);
   a.ws = reinterpret_cast<float*>(a.joins + grid);
   cudaStream_t st = (cudaStream_t)stream;
