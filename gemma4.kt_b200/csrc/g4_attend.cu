@@ -87,7 +87,7 @@ struct AttendShape {
   static constexpr int kBlockBytes = kUnit * 128;         // one block of every position
   static constexpr int kRing = kStages * kStage;
   static constexpr int kQBytes = kParts * HSP * kHeadBlock * 2;
-  static constexpr int kMeet = (kHeadBlock * HSP + kWarps * kHeadBlock * 4) * 4;  // where the warps meet; shares the fragments' memory
+  static constexpr int kMeet = kWarps * kWarps * 512;     // where the warps meet; shares the fragments' memory
   static constexpr int kSmem = kRing + (kQBytes > kMeet ? kQBytes : kMeet);
   static constexpr int kThreads = (kWarps + 1) * 32;
 };
@@ -400,14 +400,14 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   constexpr int KG = 4;  // mma steps whose operands are read together: a 128-byte block of a 16-bit head
   extern __shared__ __align__(1024) uint8_t smraw[];
   __shared__ long long red[NW + 4];
-  __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock], final_s[kHeadBlock];
+  __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock];
   __shared__ float stat[NW][kHeadBlock][2];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ unsigned boxes[NS];  // the 16-position boxes of a stage that were loaded
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs;
   const uint32_t ring = smem_u32(smraw);
   uint2* qf = reinterpret_cast<uint2*>(smraw + S::kRing);     // [part][k step][lane] B fragments of q
-  float* meet = reinterpret_cast<float*>(smraw + S::kRing);   // [head][kPitch], between items
+  float4* meet = reinterpret_cast<float4*>(smraw + S::kRing);  // [step][warp][lane], between items
   const int items = a.n_kv * a.blocks, ks = (hs + 15) / 16;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -486,16 +486,6 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   }
 
   // ---- the computing warps
-  // rows that see nothing: zeros
-  for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
-    const int seq = a.seqs[r], pos = a.pos[r];
-    if (seq < 0) continue;
-    if (seq >= a.n_seqs || pos >= a.max_positions) {
-      if (tid == 0) atomicOr(a.flags, KV_BAD_ROW);
-    } else if (pos < 0) {
-      for (int i = tid; i < a.n_kv * a.group * hs; i += NW * 32) a.out[r * a.out_stride + i] = 0.f;
-    }
-  }
   bool dead = false;  // a wait expired: no more waits, the results are void
   auto arrived = [&]() {
     if (!dead && !mbar_wait_bounded(full + stage, phase)) {
@@ -829,59 +819,65 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
       }
     }
     bar_compute<NW * 32>();  // also: every warp has read its last q fragment
-    float f[2];
+    float f[2], inv[2];
+    float* ws = a.ws + (long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock * (hs + 2);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][2 * (lane & 3) + h][0]);
-      f[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - M);
-    }
-    // All warps lay a range of dims of every head side by side, and all threads
-    // add them up; the fewer the heads, the wider the range.
-    const int heads = nh <= 1 ? 1 : nh <= 2 ? 2 : nh <= 4 ? 4 : 8;
-    const int width = min(HSP, HSP * kHeadBlock / (NW * heads)), shift = __ffs(width) - 1, pitch = width + 4;
-    if (tid < nh) {
+      const int head = 2 * (lane & 3) + h;
       float M = -INFINITY, L = 0.f;
 #pragma unroll
-      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][tid][0]);
+      for (int i = 0; i < NW; ++i) M = fmaxf(M, stat[i][head][0]);
 #pragma unroll
-      for (int i = 0; i < NW; ++i) L += stat[i][tid][0] == -INFINITY ? 0.f : exp2_approx(stat[i][tid][0] - M) * stat[i][tid][1];
-      final_s[tid] = L > 0.f ? 1.f / L : 0.f;
-      if (!whole) {
-        float* ws = a.ws + ((long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock + tid) * (hs + 2);
-        ws[0] = M;
-        ws[1] = L;
+      for (int i = 0; i < NW; ++i) L += stat[i][head][0] == -INFINITY ? 0.f : exp2_approx(stat[i][head][0] - M) * stat[i][head][1];
+      f[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - M);
+      inv[h] = !whole ? 1.f : L > 0.f ? 1.f / L : 0.f;
+      if (!whole && warp == 0 && lane < 4 && head < nh) {
+        ws[(long long)head * (hs + 2)] = M;
+        ws[(long long)head * (hs + 2) + 1] = L;
       }
     }
-    float* out = whole ? a.out + row * a.out_stride + (long long)(kvh * a.group + h0) * hs
-                       : a.ws + (long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock * (hs + 2) + 2;
+    // The same lane of every warp holds the same dims and heads: the warps lay
+    // NW steps of 16 dims side by side, each adds up and stores one of them.
+    float* out = whole ? a.out + row * a.out_stride + (long long)(kvh * a.group + h0) * hs : ws + 2;
     const int out_pitch = whole ? hs : hs + 2;
-#pragma unroll 1
-    for (int d0 = 0; d0 < ks * 16; d0 += width) {
-      if (d0) bar_compute<NW * 32>();  // the range before has been added up
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int head = 2 * (lane & 3) + h;
-        float* at = meet + (warp * heads + head) * pitch + (lane >> 2) - d0;
+    for (int i0 = 0; i0 < KS; i0 += NW) {
+      if (i0 < ks) {
+        if (i0) bar_compute<NW * 32>();  // the steps before have been added up
 #pragma unroll
-        for (int i = 0; i < KS; ++i)
-          if (head < nh && (unsigned)(i * 16 - d0) < (unsigned)width) {
-            at[i * 16] = o[i][h] * f[h];
-            at[i * 16 + 8] = o[i][2 + h] * f[h];
-          }
-      }
-      bar_compute<NW * 32>();
-      for (int e = tid; e < nh << shift; e += NW * 32) {
-        const int h = e >> shift, d = e & (width - 1);
-        float acc = 0.f;
+        for (int i = 0; i < NW; ++i)
+          meet[(i * NW + warp) * 32 + lane] = make_float4(o[i0 + i][0] * f[0], o[i0 + i][1] * f[1], o[i0 + i][2] * f[0],
+                                                          o[i0 + i][3] * f[1]);
+        bar_compute<NW * 32>();
+        float4 acc = meet[warp * NW * 32 + lane];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) acc += meet[(w * heads + h) * pitch + d];
-        if (d0 + d < hs) out[(long long)h * out_pitch + d0 + d] = whole ? acc * final_s[h] : acc;
+        for (int w = 1; w < NW; ++w) {
+          const float4 x = meet[(warp * NW + w) * 32 + lane];
+          acc.x += x.x;
+          acc.y += x.y;
+          acc.z += x.z;
+          acc.w += x.w;
+        }
+        const int d = (i0 + warp) * 16 + (lane >> 2), head = 2 * (lane & 3);
+        float* at = out + head * out_pitch + d;
+        if (head < nh && d < hs) at[0] = acc.x * inv[0];
+        if (head + 1 < nh && d < hs) at[out_pitch] = acc.y * inv[1];
+        if (head < nh && d + 8 < hs) at[8] = acc.z * inv[0];
+        if (head + 1 < nh && d + 8 < hs) at[out_pitch + 8] = acc.w * inv[1];
       }
     }
     bar_compute<NW * 32>();  // the meeting place and the statistics are free again
     first = false;
+  }
+  // rows that see nothing: zeros
+  for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+    const int seq = a.seqs[r], pos = a.pos[r];
+    if (seq < 0) continue;
+    if (seq >= a.n_seqs || pos >= a.max_positions) {
+      if (tid == 0) atomicOr(a.flags, KV_BAD_ROW);
+    } else if (pos < 0) {
+      for (int i = tid; i < a.n_kv * a.group * hs; i += NW * 32) a.out[r * a.out_stride + i] = 0.f;
+    }
   }
 }
 
