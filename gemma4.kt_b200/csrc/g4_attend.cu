@@ -881,23 +881,61 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<
   }
 }
 
-// Joins the partials of items that span CTAs. Block (c, h) belongs to the item
-// that CTA c goes on with: its CTAs but the first share the dims of head h, so
-// the longer the item, the more blocks work on it.
+// Joins the partials of items that span CTAs. A block belongs to the item that
+// the CTA of its number goes on with. Few parts: one block, its warps shared out
+// over the heads.
+// Many: the item's blocks share its heads and dims, one range of dims of one
+// head each, the longer the item the narrower.
 __global__ void __launch_bounds__(kJoinThreads) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
   __shared__ float red[kJoinThreads / 32];
   __shared__ float weight[kMaxGrid], sum[kMaxGrid];
   __shared__ __align__(8) float acc_s[2 * kJoinThreads];  // [group][dims]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs, h = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs;
   constexpr int NW = kJoinThreads / 32;
+  static_assert(NW == kHeadBlock, "a warp per head");
   grid_dep_wait();
   const int4 j = __ldcg(a.joins + blockIdx.x);
   if (j.x < 0) return;
   const int kvh = j.y / a.blocks, h0 = (j.y - kvh * a.blocks) * kHeadBlock, c = j.z >> 1, slot = j.z & 1;
-  if (h >= min(kHeadBlock, a.group - h0)) return;
-  const int n = j.w - c + 1;  // partials, in CTAs c..c + n - 1
-  const int share = (hs / 2 + n - 2) / (n - 1), d0 = 2 * share * ((int)blockIdx.x - c - 1);
-  const int per = min(share, (hs - d0) / 2);  // pairs of dims
+  const int nh = min(kHeadBlock, a.group - h0), n = j.w - c + 1;  // partials, in CTAs c..c + n - 1
+  const int task = (int)blockIdx.x - c - 1;
+  float* out = a.out + j.x * a.out_stride + (long long)(kvh * a.group + h0) * hs;
+  if (n <= kHeadBlock) {
+    const int heads = nh <= 1 ? 1 : nh <= 2 ? 2 : nh <= 4 ? 4 : 8, head = warp & (heads - 1);
+    if (task > 0 || head >= nh) return;
+    auto part = [&](int i) {
+      return a.ws + ((long long)((c + i) * 2 + (i == 0 ? slot : 0)) * kHeadBlock + head) * (hs + 2);
+    };
+    const float2 ml = lane < n ? __ldcg(reinterpret_cast<const float2*>(part(lane))) : make_float2(-INFINITY, 0.f);
+    float M = ml.x;
+#pragma unroll
+    for (int b = 4; b > 0; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
+    M = __shfl_sync(0xffffffffu, M, 0);
+    if (M == -INFINITY) M = 0.f;
+    const float w = exp2_approx(ml.x - M), L = warp_sum(w * ml.y), inv = L > 0.f ? 1.f / L : 0.f;
+    for (int d0 = warp / heads * 64; d0 < hs; d0 += NW / heads * 64) {  // (the same for every lane)
+      const int d = d0 + 2 * lane;
+      float2 v[kHeadBlock], acc = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kHeadBlock; ++i)
+        v[i] = i < n && d < hs ? __ldcg(reinterpret_cast<const float2*>(part(i) + 2 + d)) : make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kHeadBlock; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);  // 0 behind the last
+        acc.x = fmaf(wi, v[i].x, acc.x);
+        acc.y = fmaf(wi, v[i].y, acc.y);
+      }
+      if (d < hs) {
+        out[head * hs + d] = acc.x * inv;
+        out[head * hs + d + 1] = acc.y * inv;
+      }
+    }
+    return;
+  }
+  // n - 1 blocks, at least as many as heads: ranges per head (of 16 dims at least)
+  const int ranges = min((n - 1) / nh, max(1, hs / 16)), h = task / ranges, share = (hs / 2 + ranges - 1) / ranges;
+  if (h >= nh) return;
+  const int d0 = 2 * share * (task - h * ranges), per = min(share, (hs - d0) / 2);  // pairs of dims
   if (per <= 0) return;
   auto partial = [&](int i) {  // of CTA i
     return a.ws + ((long long)(i * 2 + (i == c ? slot : 0)) * kHeadBlock + h) * (hs + 2);
@@ -942,7 +980,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_attend_join_kernel(const __gr
   for (int e = tid; e < 2 * per; e += kJoinThreads) {
     float s = 0.f;
     for (int i = 0; i < min(groups, n); ++i) s += acc_s[i * 2 * per + e];
-    a.out[j.x * a.out_stride + (long long)(kvh * a.group + h0 + h) * hs + d0 + e] = L > 0.f ? s / L : 0.f;
+    out[h * hs + d0 + e] = L > 0.f ? s / L : 0.f;
   }
 }
 
@@ -1074,8 +1112,7 @@ int g4_kv_attend(g4_kv* kv, int layer, const g4_kv_queries* rows, void* work, si
   p.fn<<<grid, p.threads, p.smem, st>>>(a, kv->k_map[layer], kv->v_map[layer]);
   cudaError_t e = cudaGetLastError();
   if (!e)
-    e = launch_after(kv_attend_join_kernel, dim3(grid, a.group < kHeadBlock ? a.group : kHeadBlock), dim3(kJoinThreads),
-                     0, st, a);
+    e = launch_after(kv_attend_join_kernel, dim3(grid), dim3(kJoinThreads), 0, st, a);
   return e ? c->cuda_fail(e, "g4_kv_attend") : 0;
 }
 
