@@ -104,8 +104,10 @@ class Context:
             raise G4Error(f"g4_init({device}) failed: {msg.decode() if msg else rc}")
         self.handle = h
         self.device = device
+        self.work = {}  # work space of the paged operators, by stream
 
     def close(self) -> None:
+        self.work = {}
         if self.handle:
             lib().g4_destroy(self.handle)
             self.handle = None

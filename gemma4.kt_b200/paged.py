@@ -45,10 +45,19 @@ def _stream(device: int, stream):
 
 
 def _workspace(ctx: Context, n: int, stream):
-    """n bytes from torch's allocator, in the pool of the stream that uses them."""
+    """n bytes for a call's launches.  On torch's current stream one buffer per
+    stream is kept (calls on a stream follow one another); a call that is being
+    captured, or names its stream, gets its own from torch's allocator, in the
+    pool of the graph or stream that uses it."""
     import torch
 
     if stream is None:
+        if torch._C._cuda_getDevice() == ctx.device and not torch._C._cuda_isCurrentStreamCapturing():
+            key = torch._C._cuda_getCurrentRawStream(ctx.device)
+            kept = ctx.work.get(key)
+            if kept is None or kept.numel() < n:
+                ctx.work[key] = kept = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
+            return kept
         return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
     with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=ctx.device)):
         return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
