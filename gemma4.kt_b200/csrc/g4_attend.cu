@@ -72,12 +72,12 @@ struct AttendArgs {
 // compute, 16-position tiles per warp, stages of the ring (a stage holds a
 // unit's K or V). Two CTAs per SM share 192 KB of ring where a stage is 32 KB
 // or less; a wider head takes the SM's memory for one.
-template <int TYPE, int HSP>
+template <int TYPE, int HSP, int MT>
 struct AttendShape {
   static constexpr int kElem = TYPE == F32 ? 4 : 2;
   static constexpr int kRow = HSP * kElem;  // bytes of a position, padded
   static constexpr int kWarps = kRow > 1024 ? 2 : 4;
-  static constexpr int kTiles = kRow <= 256 ? 2 : 1;
+  static constexpr int kTiles = MT;
   static constexpr int kUnit = kWarps * kTiles * kTile;  // positions per unit
   static constexpr int kStage = kUnit * kRow;
   static constexpr int kStages = kStage <= 16384 ? 6 : 3;
@@ -390,13 +390,13 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)((c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-template <int TYPE, int HSP>
-__global__ void __launch_bounds__(AttendShape<TYPE, HSP>::kThreads, AttendShape<TYPE, HSP>::kCtas)
+template <int TYPE, int HSP, int MT>
+__global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendShape<TYPE, HSP, MT>::kCtas)
     kv_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap k_map,
                      const __grid_constant__ CUtensorMap v_map) {
-  using S = AttendShape<TYPE, HSP>;
+  using S = AttendShape<TYPE, HSP, MT>;
   constexpr bool HALF = TYPE == F16;
-  constexpr int NW = S::kWarps, MT = S::kTiles, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
+  constexpr int NW = S::kWarps, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
   constexpr int KG = 4;  // mma steps whose operands are read together: a 128-byte block of a 16-bit head
   extern __shared__ __align__(1024) uint8_t smraw[];
   __shared__ long long red[NW + 4];
@@ -990,17 +990,23 @@ struct AttendPlan {
   int threads, smem, ctas;
 };
 
-template <int TYPE, int HSP>
+template <int TYPE, int HSP, int MT>
 static AttendPlan attend_plan_s() {
-  using S = AttendShape<TYPE, HSP>;
-  return AttendPlan{kv_attend_kernel<TYPE, HSP>, S::kThreads, S::kSmem, S::kCtas};
+  using S = AttendShape<TYPE, HSP, MT>;
+  return AttendPlan{kv_attend_kernel<TYPE, HSP, MT>, S::kThreads, S::kSmem, S::kCtas};
 }
 template <int TYPE>
 static AttendPlan attend_plan_t(int hs) {
-  return hs <= 64    ? attend_plan_s<TYPE, 64>()
-         : hs <= 128 ? attend_plan_s<TYPE, 128>()
-         : hs <= 256 ? attend_plan_s<TYPE, 256>()
-                     : attend_plan_s<TYPE, 512>();
+  if (hs <= 64) return attend_plan_s<TYPE, 64, 2>();
+  // Two tiles per warp share the fragments of q and the softmax's exchange, one
+  // leaves six finer stages in the ring. Where the head's bytes fill the tile the
+  // ring decides, below that the work (64 sequences to 8000, 24 heads over 8, one
+  // against two tiles: head size 96 180 / 144 us, 112 180 / 169, 120 178 / 191,
+  // 128 181 / 187).
+  if (TYPE != F32 && hs <= 112) return attend_plan_s<TYPE, 128, 2>();
+  return hs <= 128   ? attend_plan_s<TYPE, 128, 1>()
+         : hs <= 256 ? attend_plan_s<TYPE, 256, 1>()
+                     : attend_plan_s<TYPE, 512, 1>();
 }
 static AttendPlan attend_plan(int type, int hs) {
   return type == F32 ? attend_plan_t<F32>(hs) : type == F16 ? attend_plan_t<F16>(hs) : attend_plan_t<BF16>(hs);
