@@ -244,7 +244,11 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
     float v[32];
     StripMap map{0, 0};
     const bool reads = strip.key != 0 && !done[b];  // the same in every lane
-    if (reads) map = load_strip(logits + (long long)row * stride, vocab, ((int)strip.at - b * strips) * kStrip, lane, v);
+    if (reads) {
+      map = load_strip(logits + (long long)row * stride, vocab, ((int)strip.at - b * strips) * kStrip, lane, v);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = v[i] == v[i] ? v[i] : -INFINITY;
+    }
     // the lane's largest logit, lowest token first (its elements are in token
     // order); taken, the lane looks for its next one
     float m = -INFINITY;
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
       int i_of[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const bool second = v[2 * i + 1] > v[2 * i] || !(v[2 * i] == v[2 * i]);
+        const bool second = v[2 * i + 1] > v[2 * i];
         x[i] = second ? v[2 * i + 1] : v[2 * i];
         i_of[i] = 2 * i + second;
       }
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
       for (int w = 8; w > 0; w >>= 1)
 #pragma unroll
         for (int i = 0; i < w; ++i) {
-          const bool second = x[2 * i + 1] > x[2 * i] || !(x[2 * i] == x[2 * i]);
+          const bool second = x[2 * i + 1] > x[2 * i];
           x[i] = second ? x[2 * i + 1] : x[2 * i];
           i_of[i] = second ? i_of[2 * i + 1] : i_of[2 * i];
         }
