@@ -15,9 +15,10 @@
 // Precision: activations are 32-bit.  q and p are split into parts of the
 // cache's type that sum to them (bf16: three parts of 8 bits; f16: two of 11,
 // q scaled by a power of two per head so that both parts stay normal); K and V
-// enter the mma exactly, sums are fp32.  An fp32 cache is split the same way
-// into three bf16 parts as its tile leaves shared memory, the six products
-// above 2^-24 are taken.
+// enter the mma exactly, sums are fp32.  An fp32 cache is multiplied in fp32, two
+// products an instruction, in the same places of the same threads: split into
+// parts as well it would need six mma steps for one (64 sequences to 4000, 8
+// heads over one of 256: F32US us against 100).
 //
 // Work split: the visible positions of all (row, KV head, block of 8 query
 // heads) items lie on one line, cut into equal runs of whole units (16
@@ -68,16 +69,19 @@ struct AttendArgs {
   int4* joins;              // [grid] the item that a CTA goes on with: row (-1: none), item, first CTA and its slot, last CTA
 };
 
-// Shape of one instantiation: element type, padded head size, warps that
-// compute, 16-position tiles per warp, stages of the ring (a stage holds a
-// unit's K or V). Two CTAs per SM share 192 KB of ring where a stage is 32 KB
-// or less; a wider head takes the SM's memory for one.
+// Shape of one instantiation: element type, padded head size, groups of warps
+// that own positions, 16-position tiles per group, stages of the ring (a stage
+// holds a unit's K or V). Two CTAs per SM share 192 KB of ring where a stage is
+// 32 KB or less; a wider head takes the SM's memory for one, and for an fp32
+// cache several warps split its dims, so that eight warps compute.
 template <int TYPE, int HSP, int MT>
 struct AttendShape {
   static constexpr int kElem = TYPE == F32 ? 4 : 2;
   static constexpr int kRow = HSP * kElem;  // bytes of a position, padded
-  static constexpr int kWarps = kRow > 1024 ? 2 : 4;
+  static constexpr int kWarps = kRow > 1024 ? 2 : 4;  // groups
   static constexpr int kTiles = MT;
+  static constexpr int kSplit = TYPE != F32 ? 1 : kRow > 1024 ? 4 : kRow > 512 ? 2 : 1;  // warps of a group: each its part of the dims
+  static constexpr int kAll = kWarps * kSplit;
   static constexpr int kUnit = kWarps * kTiles * kTile;  // positions per unit
   static constexpr int kStage = kUnit * kRow;
   static constexpr int kStages = kStage <= 16384 ? 6 : 3;
@@ -86,10 +90,14 @@ struct AttendShape {
   static constexpr int kBlocks = kRow / 128;              // 128-byte blocks of a row
   static constexpr int kBlockBytes = kUnit * 128;         // one block of every position
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kQBytes = kParts * HSP * kHeadBlock * 2;
-  static constexpr int kMeet = kWarps * kWarps * 512;     // where the warps meet; shares the fragments' memory
-  static constexpr int kSmem = kRing + (kQBytes > kMeet ? kQBytes : kMeet);
-  static constexpr int kThreads = (kWarps + 1) * 32;
+  // q: the parts' fragments, or (F32) rows of heads 16 bytes apart in the banks
+  static constexpr int kQPitch = HSP + 4;
+  static constexpr int kQBytes = TYPE == F32 ? kHeadBlock * kQPitch * 4 : kParts * HSP * kHeadBlock * 2;
+  static constexpr int kPBytes = TYPE == F32 ? kAll * MT * 512 : 0;  // F32: a tile's weights
+  static constexpr int kMeet = kAll * kWarps * 512;       // where the warps meet; shares the fragments' memory
+  static constexpr int kSwap = kSplit > 1 ? 2 * kAll * MT * 512 : 0;  // a group's partial scores, two units in turn
+  static constexpr int kSmem = kRing + (kQBytes + kPBytes > kMeet ? kQBytes + kPBytes : kMeet) + kSwap;
+  static constexpr int kThreads = (kAll + 1) * 32;
 };
 
 // The units of a row's visible positions: those of the first tokens, then
@@ -373,14 +381,12 @@ __device__ __forceinline__ uint32_t take_part(float& x, float& y) {
   return u;
 }
 
-// The same by truncation: three parts of 8 bits are all 24 of an fp32 number
-// exactly. For K and V on their way into the mma: integer operations, where a
-// rounding conversion of every element costs more than the products.
-__device__ __forceinline__ uint32_t cut_part(float& x, float& y) {
-  const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
-  x -= __uint_as_float(u & 0xffff0000u);
-  y -= __uint_as_float(v & 0xffff0000u);
-  return __byte_perm(u, v, 0x7632);
+// Two fp32 multiply-adds at once.
+__device__ __forceinline__ void fma2(unsigned long long& c, unsigned long long a, unsigned long long b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ float2 halves(unsigned long long x) {
+  return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
 }
 
 // Byte offset of 16-byte chunk c of position r in a stage: 128-byte blocks of
@@ -397,22 +403,41 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
   using S = AttendShape<TYPE, HSP, MT>;
   constexpr bool HALF = TYPE == F16;
   constexpr int NW = S::kWarps, NS = S::kStages, NP = S::kParts, KS = HSP / 16, BLK = S::kBlockBytes;
+  constexpr int DS = S::kSplit, NA = S::kAll, KSW = KS / DS;  // a warp's mma steps: [split * KSW, split * KSW + KSW)
   constexpr int KG = 4;  // mma steps whose operands are read together: a 128-byte block of a 16-bit head
   extern __shared__ __align__(1024) uint8_t smraw[];
-  __shared__ long long red[NW + 4];
-  __shared__ float q_unscale[kHeadBlock], q_max[NW][kHeadBlock];
+  __shared__ long long red[NA + 4];
+  __shared__ float q_unscale[kHeadBlock], q_max[NA][kHeadBlock];
   __shared__ float stat[NW][kHeadBlock][2];
   __shared__ __align__(8) uint64_t full[NS], empty[NS];
   __shared__ unsigned boxes[NS];  // the 16-position boxes of a stage that were loaded
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hs = a.hs;
+  const int group = warp / DS, split = warp % DS;
+  // F32: a lane multiplies four positions with four heads for a quarter of the
+  // dims (bits 0 and 2), and weighs four dims of 64 for the same four heads
+  // (bit 1): twice the products per load of an mma's layout, into which two
+  // exchanges bring the scores.
+  const int bit0 = lane & 1, bit2 = (lane >> 2) & 1, heads4 = (lane & 2) * 2;
+  const int dim4 = (lane >> 3) * 4 + bit2 * 2 + bit0;
+  auto four_heads = [&](const float (&f)[2], float (&all)[4]) {  // of this lane's two, in an mma's layout
+    const float x = __shfl_xor_sync(0xffffffffu, f[0], 1), y = __shfl_xor_sync(0xffffffffu, f[1], 1);
+    all[0] = bit0 ? x : f[0];
+    all[1] = bit0 ? y : f[1];
+    all[2] = bit0 ? f[0] : x;
+    all[3] = bit0 ? f[1] : y;
+  };
   const uint32_t ring = smem_u32(smraw);
   uint2* qf = reinterpret_cast<uint2*>(smraw + S::kRing);     // [part][k step][lane] B fragments of q
-  float4* meet = reinterpret_cast<float4*>(smraw + S::kRing);  // [step][warp][lane], between items
+  float* qs = reinterpret_cast<float*>(smraw + S::kRing);     // (F32) q [head][kQPitch]
+  float* weights = reinterpret_cast<float*>(smraw + S::kRing + S::kQBytes) + warp * MT * 128;  // (F32) [position][head]
+  float4* meet = reinterpret_cast<float4*>(smraw + S::kRing);  // [split][step][group][lane], between items
+  float4* swap = reinterpret_cast<float4*>(smraw + S::kSmem - S::kSwap);  // [2][group][split][tile][lane]
+  int swap_at = 0;
   const int items = a.n_kv * a.blocks, ks = (hs + 15) / 16;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(full + i, 1);
-      mbar_init(empty + i, NW);
+      mbar_init(empty + i, NA);
     }
     fence_barrier_init();
   }
@@ -431,7 +456,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
     }
   };
 
-  if (warp == NW) {
+  if (warp == NA) {
     // ---- the loading warp: lane b brings box b of every unit
     const int nblk = (hs * S::kElem + 127) / 128;
     int issued = 0;
@@ -500,7 +525,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
   };
   // q of an item's heads, as the B fragments hold it (k = dims, n = heads): the
   // values of this thread's fragment registers, read before the item begins
-  constexpr int QL = (KS + NW - 1) / NW;
+  constexpr int QL = (KS + NA - 1) / NA;
   float qv[QL][4];
   auto load_q = [&]() {
     const int kvh = k.item / a.blocks, h0 = (k.item - kvh * a.blocks) * kHeadBlock, nh = min(kHeadBlock, a.group - h0);
@@ -508,7 +533,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
     const bool vec = ((reinterpret_cast<uintptr_t>(a.q) & 7) | (a.q_stride & 1)) == 0;
 #pragma unroll
     for (int i = 0; i < QL; ++i) {
-      const int kk = warp + NW * i, h = lane >> 2, d = kk * 16 + 2 * (lane & 3);
+      const int kk = warp + NA * i, h = lane >> 2, d = kk * 16 + 2 * (lane & 3);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const float* at = q + (long long)h * hs + d + 8 * j;
@@ -539,10 +564,10 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
       if ((lane & 3) == 0) q_max[warp][lane >> 2] = m;
-      bar_compute<NW * 32>();
+      bar_compute<NA * 32>();
       m = q_max[0][lane >> 2];
 #pragma unroll
-      for (int i = 1; i < NW; ++i) m = fmaxf(m, q_max[i][lane >> 2]);
+      for (int i = 1; i < NA; ++i) m = fmaxf(m, q_max[i][lane >> 2]);
       int e = 0;
       if (m > 0.f && m < INFINITY) frexpf(m, &e);
       e = max(-100, min(100, e - 14));
@@ -555,8 +580,14 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
     }
 #pragma unroll
     for (int i = 0; i < QL; ++i) {
-      const int kk = warp + NW * i;
-      if (kk < KS)
+      const int kk = warp + NA * i;
+      if constexpr (TYPE == F32) {
+        if (kk < KS) {
+          float* at = qs + (lane >> 2) * S::kQPitch + kk * 16 + 2 * (lane & 3);
+          *reinterpret_cast<float2*>(at) = make_float2(qv[i][0], qv[i][1]);
+          *reinterpret_cast<float2*>(at + 8) = make_float2(qv[i][2], qv[i][3]);
+        }
+      } else if (kk < KS)
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           uint2 b;
@@ -565,20 +596,20 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
           qf[(p * KS + kk) * 32 + lane] = b;
         }
     }
-    bar_compute<NW * 32>();
+    bar_compute<NA * 32>();
     float sc[2];  // score factors of this thread's two heads
 #pragma unroll
     for (int j = 0; j < 2; ++j) sc[j] = a.scale_log2 * (HALF ? q_unscale[2 * (lane & 3) + j] : 1.f);
 
     // ---- the warp's tiles of every unit
-    float o[KS][4];
+    float o[KSW][4];
 #pragma unroll
-    for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < KSW; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     for (int j = 0; j < n; ++j) {
-      const int t0 = k.position(j, S::kUnit) + warp * MT * kTile;  // the warp's first position
+      const int t0 = k.position(j, S::kUnit) + group * MT * kTile;  // the group's first position
       arrived();
-      const unsigned mine = (boxes[stage] >> (warp * MT)) & ((1u << MT) - 1u);
+      const unsigned mine = (boxes[stage] >> (group * MT)) & ((1u << MT) - 1u);
       if (mine == 0) {  // nothing visible here
         release();
         arrived();
@@ -588,85 +619,137 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
       uint32_t pf[MT][NP][2];
       bool partial = false;
       {
-        // The tensor core cuts its sums off instead of rounding them, so the first
-        // parts' products, which carry the score, go into fresh sums every few steps
-        // and are added in fp32; the others' (2^-8 and less) stay in one chain each.
-        float main[MT][4], s[MT][NP][4];
+        float main[MT][4];
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < MT; ++t) main[t][0] = main[t][1] = main[t][2] = main[t][3] = 0.f;
+        if constexpr (TYPE == F32) {
+          // each product sum in two halves, even and odd dims
+          const uint8_t* kg = smraw + stage * S::kStage;
+          unsigned long long acc[MT][4][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            main[t][i] = 0.f;
+          for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int p = 0; p < NP; ++p) s[t][p][i] = 0.f;
-          }
-        const uint32_t kt = ring + stage * S::kStage;
-        const uint8_t* kg = smraw + stage * S::kStage;
-        if (TYPE != F32) {
-          // steps behind the head's end multiply what the map filled with zeros
+            for (int j = 0; j < 16; ++j) acc[t][j >> 2][j & 3] = 0ull;
+          // (chunks behind the head's end are zeros up to the block's)
 #pragma unroll 2
-          for (int k0 = 0; k0 < ks; k0 += KG) {
-            uint2 b[KG][NP];
-            uint32_t ka[KG][MT][4];
+          for (int c0 = split * KSW * 4; c0 < min(ks, (split + 1) * KSW) * 4; c0 += 4) {
+            const int c = c0 + bit2 * 2 + bit0;
+            ulonglong2 qh[4];
 #pragma unroll
-            for (int g = 0; g < KG; ++g) {
-#pragma unroll
-              for (int p = 0; p < NP; ++p) b[g][p] = qf[(p * KS + k0 + g) * 32 + lane];
-#pragma unroll
-              for (int t = 0; t < MT; ++t)
-                ldsm4(ka[g][t], kt + chunk_at<BLK>((warp * MT + t) * kTile + (lane & 15), 2 * (k0 + g) + (lane >> 4)));
-            }
-            float fresh[2][MT][4];
+            for (int h = 0; h < 4; ++h) qh[h] = *reinterpret_cast<const ulonglong2*>(qs + (heads4 + h) * S::kQPitch + 4 * c);
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) fresh[0][t][i] = fresh[1][t][i] = 0.f;
+              for (int j = 0; j < 4; ++j) {
+                const int r = (group * MT + t) * kTile + (lane >> 3) * 2 + (j & 1) + (j >> 1) * 8;
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(kg + chunk_at<BLK>(r, c));
 #pragma unroll
-            for (int g = 0; g < KG; ++g) {
+                for (int h = 0; h < 4; ++h) fma2(acc[t][j][h], x.x, qh[h].x);
 #pragma unroll
-              for (int t = 0; t < MT; ++t) mma16816<HALF>(fresh[g & 1][t], ka[g][t], b[g][0].x, b[g][0].y);
+                for (int h = 0; h < 4; ++h) fma2(acc[t][j][h], x.y, qh[h].y);
+              }
+          }
 #pragma unroll
-              for (int p = 1; p < NP; ++p)
+          for (int t = 0; t < MT; ++t) {
+            float u[4][2];  // positions j, the lane's own two heads
 #pragma unroll
-                for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][p], ka[g][t], b[g][p].x, b[g][p].y);
+            for (int j = 0; j < 4; ++j) {
+              float v[4];
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                const float2 x = halves(acc[t][j][h]);
+                v[h] = x.x + x.y;
+              }
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                u[j][e] = (bit0 ? v[2 + e] : v[e]) + __shfl_xor_sync(0xffffffffu, bit0 ? v[e] : v[2 + e], 1);
             }
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) main[t][i] += fresh[0][t][i] + fresh[1][t][i];
+              for (int e = 0; e < 2; ++e)
+                main[t][2 * r + e] = (bit2 ? u[2 * r + 1][e] : u[2 * r][e]) +
+                                     __shfl_xor_sync(0xffffffffu, bit2 ? u[2 * r][e] : u[2 * r + 1][e], 4);
           }
         } else {
-#pragma unroll 4
-          for (int kk = 0; kk < ks; ++kk) {
+          // The tensor core cuts its sums off instead of rounding them, so the first
+          // parts' products, which carry the score, go into fresh sums every few steps
+          // and are added in fp32; the others' (2^-8 and less) stay in one chain each.
+          float s[MT][NP][4];
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-              float x[8];
+          for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {  // (row, row + 8) x (col, col + 8)
-                const int r = (warp * MT + t) * kTile + (lane >> 2) + (i & 1) * 8;
-                const int c = kk * 4 + (i >> 1) * 2 + ((lane & 3) >> 1);
-                const float2 v = *reinterpret_cast<const float2*>(kg + chunk_at<BLK>(r, c) + (lane & 1) * 8);
-                x[2 * i] = v.x;
-                x[2 * i + 1] = v.y;
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+              for (int p = 0; p < NP; ++p) s[t][p][i] = 0.f;
+            }
+          const uint32_t kt = ring + stage * S::kStage;
+          {
+            // steps behind the head's end multiply what the map filled with zeros
+#pragma unroll 2
+            for (int k0 = split * KSW; k0 < min(ks, (split + 1) * KSW); k0 += KG) {
+              uint2 b[KG][NP];
+              uint32_t ka[KG][MT][4];
+#pragma unroll
+              for (int g = 0; g < KG; ++g) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) b[g][p] = qf[(p * KS + k0 + g) * 32 + lane];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                  ldsm4(ka[g][t], kt + chunk_at<BLK>((group * MT + t) * kTile + (lane & 15), 2 * (k0 + g) + (lane >> 4)));
               }
-              uint32_t ka[3][4];
+              float fresh[2][MT][4];
 #pragma unroll
-              for (int p = 0; p < 3; ++p)
+              for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) ka[p][i] = cut_part(x[2 * i], x[2 * i + 1]);
-              float fresh[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < 4; ++i) fresh[0][t][i] = fresh[1][t][i] = 0.f;
 #pragma unroll
-              for (int p = 0; p < NP; ++p) {  // products of parts i + p <= 2
-                const uint2 b = qf[(p * KS + kk) * 32 + lane];
+              for (int g = 0; g < KG; ++g) {
 #pragma unroll
-                for (int i = 0; i < 3 - p; ++i) mma16816<false>(i + p == 0 ? fresh : s[t][i], ka[i], b.x, b.y);
+                for (int t = 0; t < MT; ++t) mma16816<HALF>(fresh[g & 1][t], ka[g][t], b[g][0].x, b[g][0].y);
+#pragma unroll
+                for (int p = 1; p < NP; ++p)
+#pragma unroll
+                  for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][p], ka[g][t], b[g][p].x, b[g][p].y);
               }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) main[t][i] += fresh[i];
+              for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) main[t][i] += fresh[0][t][i] + fresh[1][t][i];
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v = s[t][NP - 1][i];
+#pragma unroll
+              for (int p = NP - 2; p >= 0; --p) v += s[t][p][i];
+              main[t][i] += v;
+            }
+        }
+        release();
+        // the sum over the group's warps
+        if (DS > 1) {
+          float4* at = swap + ((swap_at * NW + group) * DS) * MT * 32 + lane;
+          swap_at ^= 1;
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            at[(split * MT + t) * 32] = make_float4(main[t][0], main[t][1], main[t][2], main[t][3]);
+          asm volatile("bar.sync %0, %1;" ::"r"(2 + group), "n"(DS * 32) : "memory");
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            main[t][0] = main[t][1] = main[t][2] = main[t][3] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DS; ++d) {  // the same order in every warp
+              const float4 x = at[(d * MT + t) * 32];
+              main[t][0] += x.x;
+              main[t][1] += x.y;
+              main[t][2] += x.z;
+              main[t][3] += x.w;
             }
           }
         }
-        release();
         // scores: rows t0 + lane / 4 (+ 8), columns heads 2 (lane % 4) (+ 1)
         float x[MT][4], mn[2] = {m[0], m[1]};
 #pragma unroll
@@ -676,12 +759,8 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
           partial |= !whole;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float v = s[t][NP - 1][i];
-#pragma unroll
-            for (int p = NP - 2; p >= 0; --p) v += s[t][p][i];
-            v += main[t][i];
             const bool vis = whole || (have && k.seen(tt + (lane >> 2) + (i >> 1) * 8, a.sinks));
-            x[t][i] = vis ? v * sc[i & 1] : -INFINITY;
+            x[t][i] = vis ? main[t][i] * sc[i & 1] : -INFINITY;
           }
           mn[0] = fmaxf(mn[0], fmaxf(x[t][0], x[t][2]));
           mn[1] = fmaxf(mn[1], fmaxf(x[t][1], x[t][3]));
@@ -699,12 +778,21 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
             l[h] *= f[h];
             m[h] = mn[h];
           }
+          float fs[4];
+          if constexpr (TYPE == F32) four_heads(f, fs);
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            o[i][0] *= f[0];
-            o[i][1] *= f[1];
-            o[i][2] *= f[0];
-            o[i][3] *= f[1];
+          for (int i = 0; i < KSW; ++i) {
+            if constexpr (TYPE == F32) {  // a dim's four heads
+              o[i][0] *= fs[0];
+              o[i][1] *= fs[1];
+              o[i][2] *= fs[2];
+              o[i][3] *= fs[3];
+            } else {  // two dims' two heads
+              o[i][0] *= f[0];
+              o[i][1] *= f[1];
+              o[i][2] *= f[0];
+              o[i][3] *= f[1];
+            }
           }
         }
 #pragma unroll
@@ -716,23 +804,30 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
             x[t][i] = exp2_approx(x[t][i] - mm + (HALF ? 8.f : 0.f));
             l[i & 1] += x[t][i];
           }
+          if constexpr (TYPE == F32) {
+            float2* at = reinterpret_cast<float2*>(weights + (t * kTile + (lane >> 2)) * 8) + (lane & 3);
+            at[0] = make_float2(x[t][0], x[t][1]);
+            at[8 * 4] = make_float2(x[t][2], x[t][3]);
+          } else {
 #pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            pf[t][p][0] = transpose8(take_part<HALF>(x[t][0], x[t][1]));
-            pf[t][p][1] = transpose8(take_part<HALF>(x[t][2], x[t][3]));
+            for (int p = 0; p < NP; ++p) {
+              pf[t][p][0] = transpose8(take_part<HALF>(x[t][0], x[t][1]));
+              pf[t][p][1] = transpose8(take_part<HALF>(x[t][2], x[t][3]));
+            }
           }
         }
       }
       arrived();
+      if (TYPE == F32) __syncwarp();  // the weights are there
       {
         const uint32_t vt = ring + stage * S::kStage;
         const uint8_t* vg = smraw + stage * S::kStage;
-        if (partial) {  // V rows that are not seen become zeros
+        if (partial) {  // V rows that are not seen become zeros (the warp's dims of them)
           for (int e = lane; e < MT * kTile * 8; e += 32) {
             const int r = e >> 3, t = t0 + r;
             if (!((mine >> (r / kTile)) & 1u) || !k.seen(t, a.sinks))
-              for (int b = 0; b < (ks * S::kElem + 7) / 8; ++b)
-                *reinterpret_cast<uint4*>(smraw + stage * S::kStage + b * BLK + (warp * MT * kTile + r) * 128 + (e & 7) * 16) =
+              for (int b = split * (KSW * S::kElem / 8); b < min((ks * S::kElem + 7) / 8, (split + 1) * (KSW * S::kElem / 8)); ++b)
+                *reinterpret_cast<uint4*>(smraw + stage * S::kStage + b * BLK + (group * MT * kTile + r) * 128 + (e & 7) * 16) =
                     make_uint4(0, 0, 0, 0);
           }
           // ordered before the stage's next load, which another proxy writes
@@ -742,18 +837,18 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
         // (a tile's sums are fresh, too, and added to O in fp32)
         if (TYPE != F32) {
 #pragma unroll
-          for (int i = 0; i < KS; i += KG) {
-            if (i < ks) {
+          for (int i = 0; i < KSW; i += KG) {
+            if (split * KSW + i < ks) {
               float fresh[KG][4];
 #pragma unroll
               for (int g = 0; g < KG; ++g) fresh[g][0] = fresh[g][1] = fresh[g][2] = fresh[g][3] = 0.f;
 #pragma unroll
               for (int t = 0; t < MT; ++t) {
                 uint32_t va[KG][4];
-                const int r = (warp * MT + t) * kTile + (lane & 7) + (lane >> 4) * 8;
+                const int r = (group * MT + t) * kTile + (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
                 for (int g = 0; g < KG; ++g)
-                  ldsm4_t(va[g], vt + chunk_at<BLK>(r, 2 * (i + g) + ((lane >> 3) & 1)));
+                  ldsm4_t(va[g], vt + chunk_at<BLK>(r, 2 * (split * KSW + i + g) + ((lane >> 3) & 1)));
 #pragma unroll
                 for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
@@ -766,34 +861,40 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
             }
           }
         } else {
+          // o[4 g + d] are the lane's four heads of its dim d of the g-th 64
+          unsigned long long acc[KSW][2];
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            if (i < ks) {
-              float fresh[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int i = 0; i < KSW; ++i)
 #pragma unroll
-              for (int t = 0; t < MT; ++t) {
-                // V[pos 2 (lane % 4) + {0, 1} (+ 8)][dim lane / 4 (+ 8)]: registers (dim), (dim + 8), then pos + 8
-                float x[8];
+            for (int e = 0; e < 2; ++e)
+              acc[i][e] = (unsigned long long)__float_as_uint(o[i][2 * e]) |
+                          (unsigned long long)__float_as_uint(o[i][2 * e + 1]) << 32;
+#pragma unroll 4
+          for (int p = 0; p < MT * kTile; ++p) {
+            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(weights + p * 8 + heads4);
+            const int r = group * MT * kTile + p;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const int r = (warp * MT + t) * kTile + 2 * (lane & 3) + (e & 1) + (e >> 2) * 8;
-                  const int d = i * 16 + (lane >> 2) + ((e >> 1) & 1) * 8;
-                  x[e] = *reinterpret_cast<const float*>(vg + chunk_at<BLK>(r, d >> 2) + (d & 3) * 4);
+            for (int g = 0; g < KSW / 4; ++g) {
+              if (split * KSW * 16 + g * 64 < hs) {
+                const uint4 x = *reinterpret_cast<const uint4*>(vg + chunk_at<BLK>(r, split * KSW * 4 + g * 16 + dim4));
+                const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                  const unsigned long long vv = (unsigned long long)v[d] | (unsigned long long)v[d] << 32;
+                  fma2(acc[4 * g + d][0], vv, w.x);
+                  fma2(acc[4 * g + d][1], vv, w.y);
                 }
-                uint32_t va[3][4];
-#pragma unroll
-                for (int p = 0; p < 3; ++p)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) va[p][e] = cut_part(x[2 * e], x[2 * e + 1]);
-#pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
-#pragma unroll
-                  for (int e = 2 - p; e >= 0; --e) mma16816<false>(fresh, va[e], pf[t][p][0], pf[t][p][1]);
               }
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[i][e] += fresh[e];
             }
           }
+#pragma unroll
+          for (int i = 0; i < KSW; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float2 y = halves(acc[i][e]);
+              o[i][2 * e] = y.x;
+              o[i][2 * e + 1] = y.y;
+            }
         }
       }
       release();
@@ -813,12 +914,12 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int b = 4; b < 32; b <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], b);
-      if (lane < 4) {
-        stat[warp][2 * lane + h][0] = m[h];
-        stat[warp][2 * lane + h][1] = l[h];
+      if (split == 0 && lane < 4) {  // (a group's warps have the same)
+        stat[group][2 * lane + h][0] = m[h];
+        stat[group][2 * lane + h][1] = l[h];
       }
     }
-    bar_compute<NW * 32>();  // also: every warp has read its last q fragment
+    bar_compute<NA * 32>();  // also: every warp has read its last q fragment
     float f[2], inv[2];
     float* ws = a.ws + (long long)(blockIdx.x * 2 + (first ? 0 : 1)) * kHeadBlock * (hs + 2);
 #pragma unroll
@@ -836,29 +937,48 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
         ws[(long long)head * (hs + 2) + 1] = L;
       }
     }
-    // The same lane of every warp holds the same dims and heads: the warps lay
-    // NW steps of 16 dims side by side, each adds up and stores one of them.
+    // The same lane of every group's warp for a part of the dims holds the same
+    // dims and heads: they lay NW steps of 16 dims side by side, each adds up and
+    // stores one of them.
+    float fs[4], invs[4];
+    if constexpr (TYPE == F32) {
+      four_heads(f, fs);
+      four_heads(inv, invs);
+    }
+    float4* mine_at = meet + split * (NW * NW * 32);
     float* out = whole ? a.out + row * a.out_stride + (long long)(kvh * a.group + h0) * hs : ws + 2;
     const int out_pitch = whole ? hs : hs + 2;
 #pragma unroll
-    for (int i0 = 0; i0 < KS; i0 += NW) {
-      if (i0 < ks) {
-        if (i0) bar_compute<NW * 32>();  // the steps before have been added up
+    for (int i0 = 0; i0 < KSW; i0 += NW) {
+      if (i0 < ks) {  // (the same for all warps)
+        if (i0) bar_compute<NA * 32>();  // the steps before have been added up
 #pragma unroll
         for (int i = 0; i < NW; ++i)
-          meet[(i * NW + warp) * 32 + lane] = make_float4(o[i0 + i][0] * f[0], o[i0 + i][1] * f[1], o[i0 + i][2] * f[0],
-                                                          o[i0 + i][3] * f[1]);
-        bar_compute<NW * 32>();
-        float4 acc = meet[warp * NW * 32 + lane];
+          mine_at[(i * NW + group) * 32 + lane] =
+              TYPE == F32 ? make_float4(o[i0 + i][0] * fs[0], o[i0 + i][1] * fs[1], o[i0 + i][2] * fs[2], o[i0 + i][3] * fs[3])
+                          : make_float4(o[i0 + i][0] * f[0], o[i0 + i][1] * f[1], o[i0 + i][2] * f[0], o[i0 + i][3] * f[1]);
+        bar_compute<NA * 32>();
+        float4 acc = mine_at[group * NW * 32 + lane];
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
-          const float4 x = meet[(warp * NW + w) * 32 + lane];
+          const float4 x = mine_at[(group * NW + w) * 32 + lane];
           acc.x += x.x;
           acc.y += x.y;
           acc.z += x.z;
           acc.w += x.w;
         }
-        const int d = (i0 + warp) * 16 + (lane >> 2), head = 2 * (lane & 3);
+        if constexpr (TYPE == F32) {
+          const int i = i0 + group, d = split * KSW * 16 + (i >> 2) * 64 + dim4 * 4 + (i & 3);
+          float* at = out + heads4 * out_pitch + d;
+          if (d < hs) {
+            if (heads4 < nh) at[0] = acc.x * invs[0];
+            if (heads4 + 1 < nh) at[out_pitch] = acc.y * invs[1];
+            if (heads4 + 2 < nh) at[2 * out_pitch] = acc.z * invs[2];
+            if (heads4 + 3 < nh) at[3 * out_pitch] = acc.w * invs[3];
+          }
+          continue;
+        }
+        const int d = (split * KSW + i0 + group) * 16 + (lane >> 2), head = 2 * (lane & 3);
         float* at = out + head * out_pitch + d;
         if (head < nh && d < hs) at[0] = acc.x * inv[0];
         if (head + 1 < nh && d < hs) at[out_pitch] = acc.y * inv[1];
@@ -866,7 +986,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
         if (head + 1 < nh && d + 8 < hs) at[out_pitch + 8] = acc.w * inv[1];
       }
     }
-    bar_compute<NW * 32>();  // the meeting place and the statistics are free again
+    bar_compute<NA * 32>();  // the meeting place and the statistics are free again
     first = false;
   }
   // rows that see nothing: zeros
@@ -876,7 +996,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
     if (seq >= a.n_seqs || pos >= a.max_positions) {
       if (tid == 0) atomicOr(a.flags, KV_BAD_ROW);
     } else if (pos < 0) {
-      for (int i = tid; i < a.n_kv * a.group * hs; i += NW * 32) a.out[r * a.out_stride + i] = 0.f;
+      for (int i = tid; i < a.n_kv * a.group * hs; i += NA * 32) a.out[r * a.out_stride + i] = 0.f;
     }
   }
 }
@@ -1003,7 +1123,8 @@ static AttendPlan attend_plan_t(int hs) {
   // ring decides, below that the work (64 sequences to 8000, 24 heads over 8, one
   // against two tiles: head size 96 180 / 144 us, 112 180 / 169, 120 178 / 191,
   // 128 181 / 187).
-  if (TYPE != F32 && hs <= 112) return attend_plan_s<TYPE, 128, 2>();
+  if constexpr (TYPE != F32)
+    if (hs <= 112) return attend_plan_s<TYPE, 128, 2>();
   return hs <= 128   ? attend_plan_s<TYPE, 128, 1>()
          : hs <= 256 ? attend_plan_s<TYPE, 256, 1>()
                      : attend_plan_s<TYPE, 512, 1>();
