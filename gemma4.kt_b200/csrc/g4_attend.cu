@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[t][j >> 2][j & 3] = 0ull;
           // (chunks behind the head's end are zeros up to the block's)
-#pragma unroll 2
+#pragma unroll 4
           for (int c0 = split * KSW * 4; c0 < min(ks, (split + 1) * KSW) * 4; c0 += 4) {
             const int c = c0 + bit2 * 2 + bit0;
             ulonglong2 qh[4];
@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
             for (int e = 0; e < 2; ++e)
               acc[i][e] = (unsigned long long)__float_as_uint(o[i][2 * e]) |
                           (unsigned long long)__float_as_uint(o[i][2 * e + 1]) << 32;
-#pragma unroll 4
+#pragma unroll 8
           for (int p = 0; p < MT * kTile; ++p) {
             const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(weights + p * 8 + heads4);
             const int r = group * MT * kTile + p;
