@@ -15,10 +15,12 @@
 // Precision: activations are 32-bit.  q and p are split into parts of the
 // cache's type that sum to them (bf16: three parts of 8 bits; f16: two of 11,
 // q scaled by a power of two per head so that both parts stay normal); K and V
-// enter the mma exactly, sums are fp32.  An fp32 cache is multiplied in fp32, two
-// products an instruction, in the same places of the same threads: split into
-// parts as well it would need six mma steps for one (64 sequences to 4000, 8
-// heads over one of 256: F32US us against 100).
+// enter the mma exactly.  The tensor core cuts its sums off: they are taken
+// fresh every few steps and added in fp32 (without: 1e-6 to 3e-6 of the result
+// off, growing with the context; with: 2e-7 to 5e-7, less than fp32 matrix
+// products).  An fp32 cache is multiplied in fp32, two products an instruction:
+// K and V split into parts as well would need six mma steps for one (64
+// sequences to 4000, 8 heads over one of 256: 106 us against 83).
 //
 // Work split: the visible positions of all (row, KV head, block of 8 query
 // heads) items lie on one line, cut into equal runs of whole units (16
@@ -27,6 +29,12 @@
 // alike keep every SM busy and a captured launch stays right when the
 // positions change.  Runs that end inside an item leave (max, sum, O) partials
 // in the caller's work space; a second launch joins them in a fixed order.
+//
+// Bound where: 96 ragged sequences to 12001 (64 heads over 8 of 128, bf16) run
+// at the measured copy rate (357 us for 2.37 GB), one of 131071 (f16) at 96% of
+// it; 64 sequences with a window of 512 (16 heads over 8 of 256, bf16) at 73%:
+// what is left is the start of a run (position, page, first bytes: 4 us) and
+// the join (3 us). A call of a few positions takes 8 to 13 us.
 //
 // Inside a run one warp brings units in (TMA boxes of 16 positions x 128 bytes
 // of a head, swizzled so that fragment loads hit distinct banks; K and V of a
@@ -679,44 +687,39 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
 #pragma unroll
           for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-#pragma unroll
-              for (int p = 0; p < NP; ++p) s[t][p][i] = 0.f;
-            }
+            for (int p = 0; p < NP; ++p) s[t][p][0] = s[t][p][1] = s[t][p][2] = s[t][p][3] = 0.f;
           const uint32_t kt = ring + stage * S::kStage;
-          {
-            // steps behind the head's end multiply what the map filled with zeros
+          // steps behind the head's end multiply what the map filled with zeros
 #pragma unroll 2
-            for (int k0 = split * KSW; k0 < min(ks, (split + 1) * KSW); k0 += KG) {
-              uint2 b[KG][NP];
-              uint32_t ka[KG][MT][4];
+          for (int k0 = split * KSW; k0 < min(ks, (split + 1) * KSW); k0 += KG) {
+            uint2 b[KG][NP];
+            uint32_t ka[KG][MT][4];
 #pragma unroll
-              for (int g = 0; g < KG; ++g) {
+            for (int g = 0; g < KG; ++g) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) b[g][p] = qf[(p * KS + k0 + g) * 32 + lane];
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-                  ldsm4(ka[g][t], kt + chunk_at<BLK>((group * MT + t) * kTile + (lane & 15), 2 * (k0 + g) + (lane >> 4)));
-              }
-              float fresh[2][MT][4];
+              for (int p = 0; p < NP; ++p) b[g][p] = qf[(p * KS + k0 + g) * 32 + lane];
 #pragma unroll
               for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) fresh[0][t][i] = fresh[1][t][i] = 0.f;
-#pragma unroll
-              for (int g = 0; g < KG; ++g) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t) mma16816<HALF>(fresh[g & 1][t], ka[g][t], b[g][0].x, b[g][0].y);
-#pragma unroll
-                for (int p = 1; p < NP; ++p)
-#pragma unroll
-                  for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][p], ka[g][t], b[g][p].x, b[g][p].y);
-              }
-#pragma unroll
-              for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) main[t][i] += fresh[0][t][i] + fresh[1][t][i];
+                ldsm4(ka[g][t], kt + chunk_at<BLK>((group * MT + t) * kTile + (lane & 15), 2 * (k0 + g) + (lane >> 4)));
             }
+            float fresh[2][MT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) fresh[0][t][i] = fresh[1][t][i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < KG; ++g) {
+#pragma unroll
+              for (int t = 0; t < MT; ++t) mma16816<HALF>(fresh[g & 1][t], ka[g][t], b[g][0].x, b[g][0].y);
+#pragma unroll
+              for (int p = 1; p < NP; ++p)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) mma16816<HALF>(s[t][p], ka[g][t], b[g][p].x, b[g][p].y);
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) main[t][i] += fresh[0][t][i] + fresh[1][t][i];
           }
 #pragma unroll
           for (int t = 0; t < MT; ++t)
