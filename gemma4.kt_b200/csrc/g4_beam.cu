@@ -24,7 +24,7 @@ namespace g4 {
 constexpr int kScanThreads = 128;
 constexpr int kStrip = 1024;  // logits per warp: 32 per lane, 4 KB in flight
 constexpr int kMaxBeams = 32;
-constexpr int kPickThreads = 512;
+constexpr int kPickThreads = 1024;
 
 // exp(v) is taken as 2^(v * kLog2e) with this rounded constant throughout, and
 // the logarithm divided by the same one, so its rounding does not enter.
