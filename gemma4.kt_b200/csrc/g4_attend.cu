@@ -31,7 +31,7 @@
 // in the caller's work space; a second launch joins them in a fixed order.
 //
 // Bound where: 96 ragged sequences to 12001 (64 heads over 8 of 128, bf16) run
-// at the measured copy rate (357 us for 2.37 GB), one of 131071 (f16) at 96% of
+// at the measured copy rate (353 us for 2.37 GB), one of 131071 (f16) at 90% of
 // it; 64 sequences with a window of 512 (16 heads over 8 of 256, bf16) at 73%:
 // what is left is the start of a run (position, page, first bytes: 4 us) and
 // the join (3 us). A call of a few positions takes 8 to 13 us.
@@ -56,6 +56,8 @@ namespace g4 {
 constexpr int kHeadBlock = 8;  // query heads per item: the mma's columns
 constexpr int kTile = 16;      // positions per warp and step: the mma's rows
 constexpr int kJoinThreads = 256;
+// What an item counts beside its units in the work split (0 / 1 / 2: 64 windowed
+// sequences 63 / 51 / 52 us, 128 of 10 to 300 positions 38 / 31 / 30).
 constexpr int kItemUnits = 1;
 constexpr int kMaxGrid = 512;  // CTAs (a B200 takes 296)
 static_assert(kKvMaxHeadSize <= 2 * kJoinThreads, "two dims per thread of the join");
@@ -1118,17 +1120,14 @@ static AttendPlan attend_plan_s() {
   using S = AttendShape<TYPE, HSP, MT>;
   return AttendPlan{kv_attend_kernel<TYPE, HSP, MT>, S::kThreads, S::kSmem, S::kCtas};
 }
+// Two tiles per warp share the fragments of q and the softmax's exchange; one
+// leaves finer stages in the ring. For short rows the work decides: under the
+// power cap of a long run 96 sequences to 12001 (bf16, heads of 128) take 352 us
+// with two and 404 with one, although a short burst takes 354 and 360.
 template <int TYPE>
 static AttendPlan attend_plan_t(int hs) {
-  if (hs <= 64) return attend_plan_s<TYPE, 64, 2>();
-  // Two tiles per warp share the fragments of q and the softmax's exchange, one
-  // leaves six finer stages in the ring. Where the head's bytes fill the tile the
-  // ring decides, below that the work (64 sequences to 8000, 24 heads over 8, one
-  // against two tiles: head size 96 180 / 144 us, 112 180 / 169, 120 178 / 191,
-  // 128 181 / 187).
-  if constexpr (TYPE != F32)
-    if (hs <= 112) return attend_plan_s<TYPE, 128, 2>();
-  return hs <= 128   ? attend_plan_s<TYPE, 128, 1>()
+  return hs <= 64    ? attend_plan_s<TYPE, 64, 2>()
+         : hs <= 128 ? attend_plan_s<TYPE, 128, TYPE == F32 ? 1 : 2>()
          : hs <= 256 ? attend_plan_s<TYPE, 256, 1>()
                      : attend_plan_s<TYPE, 512, 1>();
 }
