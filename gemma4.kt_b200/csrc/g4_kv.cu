@@ -14,7 +14,9 @@
 // (4 bytes a page; 64 K pages are 256 KB) and their cost is latency, not
 // bandwidth.  What is bound by HBM is the copying, one warp per (page, layer,
 // K or V, head) strip of consecutive bytes, eight 16-byte loads in flight per
-// lane.
+// lane: 1001 pages of 256 KB in 81 us (6.5 TB/s read and written, the measured
+// copy rate), 64 shared last pages over 8 layers in 12 us. A fork takes 3 to 4 us,
+// planning a resize or a compaction 4 to 6 (thousands of pages).
 #include "g4_common.cuh"
 #include "g4_kv.h"
 
