@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -52,7 +53,7 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 def build_cuda(verbose: bool = False) -> Path:
     OUT.mkdir(exist_ok=True)
     headers = [CSRC / h for h in CU_HEADERS] + [INCLUDE / "g4.h"]
-    objs = []
+    objs, steps = [], []
     for src in CU_SOURCES:
         s = CSRC / src
         if not s.exists():
@@ -62,8 +63,10 @@ def build_cuda(verbose: bool = False) -> Path:
             cmd = [NVCC, *NVCC_FLAGS, "-c", str(s), "-o", str(o)]
             if verbose:
                 cmd.insert(1, "-Xptxas=-v")
-            _run(cmd)
+            steps.append(cmd)
         objs.append(o)
+    with ThreadPoolExecutor(max(1, min(len(steps), os.cpu_count() or 1))) as pool:
+        list(pool.map(_run, steps))  # one compiler per source; the first failure is raised
     lib = PKG / "libg4b200.so"
     if _stale(lib, objs):
         _run([NVCC, *ARCH, "-shared", "-o", str(lib), *map(str, objs), "-ldl", "-lcudart"])
