@@ -629,9 +629,9 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
       uint32_t pf[MT][NP][2];
       bool partial = false;
       {
-        float main[MT][4];
+        float score[MT][4];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) main[t][0] = main[t][1] = main[t][2] = main[t][3] = 0.f;
+        for (int t = 0; t < MT; ++t) score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.f;
         if constexpr (TYPE == F32) {
           // each product sum in two halves, even and odd dims
           const uint8_t* kg = smraw + stage * S::kStage;
@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
             for (int r = 0; r < 2; ++r)
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                main[t][2 * r + e] = (bit2 ? u[2 * r + 1][e] : u[2 * r][e]) +
+                score[t][2 * r + e] = (bit2 ? u[2 * r + 1][e] : u[2 * r][e]) +
                                      __shfl_xor_sync(0xffffffffu, bit2 ? u[2 * r][e] : u[2 * r + 1][e], 4);
           }
         } else {
@@ -721,7 +721,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) main[t][i] += fresh[0][t][i] + fresh[1][t][i];
+              for (int i = 0; i < 4; ++i) score[t][i] += fresh[0][t][i] + fresh[1][t][i];
           }
 #pragma unroll
           for (int t = 0; t < MT; ++t)
@@ -730,7 +730,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
               float v = s[t][NP - 1][i];
 #pragma unroll
               for (int p = NP - 2; p >= 0; --p) v += s[t][p][i];
-              main[t][i] += v;
+              score[t][i] += v;
             }
         }
         release();
@@ -740,18 +740,18 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
           swap_at ^= 1;
 #pragma unroll
           for (int t = 0; t < MT; ++t)
-            at[(split * MT + t) * 32] = make_float4(main[t][0], main[t][1], main[t][2], main[t][3]);
+            at[(split * MT + t) * 32] = make_float4(score[t][0], score[t][1], score[t][2], score[t][3]);
           asm volatile("bar.sync %0, %1;" ::"r"(2 + group), "n"(DS * 32) : "memory");
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
-            main[t][0] = main[t][1] = main[t][2] = main[t][3] = 0.f;
+            score[t][0] = score[t][1] = score[t][2] = score[t][3] = 0.f;
 #pragma unroll
             for (int d = 0; d < DS; ++d) {  // the same order in every warp
               const float4 x = at[(d * MT + t) * 32];
-              main[t][0] += x.x;
-              main[t][1] += x.y;
-              main[t][2] += x.z;
-              main[t][3] += x.w;
+              score[t][0] += x.x;
+              score[t][1] += x.y;
+              score[t][2] += x.z;
+              score[t][3] += x.w;
             }
           }
         }
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const bool vis = whole || (have && k.seen(tt + (lane >> 2) + (i >> 1) * 8, a.sinks));
-            x[t][i] = vis ? main[t][i] * sc[i & 1] : -INFINITY;
+            x[t][i] = vis ? score[t][i] * sc[i & 1] : -INFINITY;
           }
           mn[0] = fmaxf(mn[0], fmaxf(x[t][0], x[t][2]));
           mn[1] = fmaxf(mn[1], fmaxf(x[t][1], x[t][3]));

@@ -50,6 +50,24 @@ def test_paged_batch_vs_oracle(g4, ctx, name, page):
     model.free()
 
 
+def test_paged_batch_moe(g4, ctx, monkeypatch):
+    """MoE layers beside the paged attention (the fp32 expert kernels, as in the
+    contiguous batch's test)."""
+    monkeypatch.setenv("G4_MOE_TC", "0")
+    m, src, model, _ = _models(g4, ctx, SPECS["moe"], seed=39)
+    batch = model.new_paged_batch(2, 32, page_size=16)
+    orcs = [oracle.ModelOracle(src) for _ in range(2)]
+    prompts = [np.concatenate([[2], m.prompt(11, seed=6000 + i)]) for i in range(2)]
+    for p in range(12):
+        lg, _ = batch.step([int(t[p]) for t in prompts], [p, p])
+        for i in range(2):
+            assert rel_l2(lg[i], orcs[i].step(int(prompts[i][p]), p)) < TOL, (i, p)
+    for o in orcs:
+        o.close()
+    batch.free()
+    model.free()
+
+
 def test_paged_prefill_and_forks(g4, ctx):
     """One prompt in chunks that cross page borders, three slots forked from it,
     each going its own way: the shared pages stay, the last one is copied."""

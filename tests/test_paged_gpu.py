@@ -253,7 +253,7 @@ def test_rope_scaling(g4, ctx, scaling, kw):
 @pytest.mark.parametrize("hs,heads,kv,rows,norm,layout,rot", [
     (64, 4, 2, 1, True, "half", 64), (128, 5, 1, 70, False, "interleaved", 64), (256, 16, 8, 9, True, "half", 256),
     (72, 3, 3, 33, True, "interleaved", 72), (512, 2, 1, 5, True, "half", 128), (64, 8, 8, 2500, False, "half", 64),
-    (8, 1, 1, 17, False, "half", None)])
+    (8, 1, 1, 17, False, "half", None), (136, 6, 3, 40, True, "half", None), (512, 4, 2, 700, True, "interleaved", 512)])
 def test_append(g4, ctx, kind, hs, heads, kv, rows, norm, layout, rot):
     page, n_seq = 32, 3
     positions = rows + 100
@@ -453,6 +453,55 @@ def test_attend_offsets_beyond_32_bits(g4, ctx):
     cache.copy_pages(i32([page]), i32([0]))
     assert torch.equal(cache.k(0)[0].view(torch.int16), cache.k(0)[page].view(torch.int16))
     cache.free()
+
+
+def test_attend_leaves_missing_pages_out(g4, ctx):
+    """A visible position without a page is reported, and the rest is attended."""
+    for kind in ("f32", "bf16"):
+        cache = new_cache(g4, ctx, kind, (1,), (64,), 16, 16, 2, 256)
+        cache.resize(i32([0]), i32([160]))
+        g = torch.Generator(device="cuda").manual_seed(6)
+        for p in (cache.k(0), cache.v(0)):
+            p.copy_(torch.randn(p.shape, generator=g, device="cuda"))
+        q, out = torch.randn(1, 256, generator=g, device="cuda"), torch.empty(1, 256, device="cuda")
+        table = host(cache.table)
+        cache.table[0, 3] = -1
+        cache.table[0, 7] = 16  # no such page
+        cache.attend(0, q, out, i32([0]), i32([150]), scale=0.1)
+        with pytest.raises(g4.G4Error, match="without a page"):
+            cache.check()
+        t = np.array([t for t in range(151) if t // 16 not in (3, 7)])
+        k, v = (host(p)[table[0, t // 16], 0, t % 16] for p in (cache.k(0), cache.v(0)))
+        x = 0.1 * host(q).reshape(4, 64) @ k.T
+        p = np.exp(x - x.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        # the bound of paged_ref.attend
+        dx = (64 / 16 + 6) * 2.0 ** -23 * (0.1 * abs(host(q)).reshape(4, 64) @ abs(k).T).max(1) + 2.0 ** -22
+        bound = (p @ abs(v)) * (2 * dx[:, None] + (len(t) / 64 + 16) * 2.0 ** -23)
+        assert np.all(abs(host(out).reshape(4, 64) - p @ v) <= bound)
+
+
+def test_most_sequences(g4, ctx):
+    """The largest number of sequences and entries."""
+    n = 4096
+    cache = new_cache(g4, ctx, kv=(1,), hs=(8,), pages=2 * n, seqs=n, positions=64)
+    sim = mirrored(cache)
+    rng = np.random.default_rng(11)
+    lens = rng.integers(0, 33, n)
+    order = rng.permutation(n)
+    cache.resize(i32(order), i32(lens))
+    assert sim.resize(order, lens)
+    src = rng.permutation(n)
+    cache.fork(i32(src), i32(order))
+    sim.fork(src, order)
+    same_state(cache, sim)
+    cache.compact()
+    sim.compact()
+    same_state(cache, sim)
+    cache.resize(i32(order), i32([0] * n))
+    assert cache.check() == 2 * n
+    with pytest.raises(g4.G4Error):
+        cache.fork(i32([0] * (n + 1)), i32([0] * (n + 1)))
 
 
 def test_attend_reports_bad_rows(g4, ctx):
