@@ -32,11 +32,15 @@ constexpr int kStrip = 1024;  // logits per warp: 32 per lane, 4 KB in flight
 constexpr int kMaxBeams = 32;
 constexpr int kPickThreads = 1024;
 
-// exp(v) is taken as 2^(v * kLog2e) with this rounded constant throughout, and
-// the logarithm divided by the same one, so its rounding does not enter.
+// exp(v - m) is taken as 2^((v - m) * kLog2e) with this rounded constant
+// throughout, and the logarithm divided by the same one. The maximum is
+// subtracted before the factor: a product of a logit of -1e10 is rounded by
+// hundreds, one of 2.4e38 is infinite, and such logits are how a vocabulary is
+// masked; a difference is exact next to the maximum, and one that overflows is
+// -inf, whose term is 0. Every finite strip's sum is then 1 to kStrip.
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A strip: its largest logit m (-inf: none) and the sum of 2^(v * kLog2e - m * kLog2e).
+// A strip: its largest logit m (-inf: none) and the sum of 2^((v - m) * kLog2e).
 struct StripStat {
   float m, sum;
 };
@@ -108,15 +112,15 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const float* lo
     m1 = fmaxf(m1, v[i + 1]);
   }
   const float m = value_of(__reduce_max_sync(0xffffffffu, order_of(fmaxf(m0, m1))));
-  const float c = m == -INFINITY ? 0.f : __fmul_rn(m, kLog2e);
+  const float base = m == -INFINITY ? 0.f : m;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i & 3] += beam_exp2(fmaf(v[i], kLog2e, -c));
+  for (int i = 0; i < 32; ++i) s[i & 3] += beam_exp2((v[i] - base) * kLog2e);
   float sum = (s[0] + s[1]) + (s[2] + s[3]);
   if (!(sum == sum)) {  // NaNs count as masked
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) sum += v[i] == v[i] ? beam_exp2(fmaf(v[i], kLog2e, -c)) : 0.f;
+    for (int i = 0; i < 32; ++i) sum += v[i] == v[i] ? beam_exp2((v[i] - base) * kLog2e) : 0.f;
   }
   sum = warp_sum(sum);
   if (lane == 0) stats[w] = StripStat{m, sum};
@@ -158,7 +162,10 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
     const int32_t* finished, int beams, int strips, int pad_token, float* new_scores, int32_t* parents,
     int32_t* tokens) {
   constexpr int NW = kPickThreads / 32;
-  __shared__ double lse[kMaxBeams], score_of[kMaxBeams];
+  // a row's largest logit and the logarithm of its sum relative to that one. A log
+  // probability is (logit - largest) - logarithm: their sum would lose the
+  // logarithm beside a largest logit of -1e20, where nothing of a row is live.
+  __shared__ double largest[kMaxBeams], log_sum[kMaxBeams], score_of[kMaxBeams];
   __shared__ int done[kMaxBeams];
   __shared__ Ranked lists[NW * kMaxBeams];
   __shared__ Ranked chosen[kMaxBeams];
@@ -187,10 +194,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
     for (int i = lane + 32 * kHold; i < strips; i += 32) M = fmaxf(M, st[i].m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float C = __fmul_rn(M, kLog2e);
-    auto part = [&](const StripStat& t) {
-      return t.m > -INFINITY ? t.sum * beam_exp2(__fmul_rn(t.m, kLog2e) - C) : 0.f;
-    };
+    auto part = [&](const StripStat& t) { return t.m > -INFINITY ? t.sum * beam_exp2((t.m - M) * kLog2e) : 0.f; };
     float near = 0.f;
 #pragma unroll
     for (int i = 0; i < kHold; ++i) near += part(x[i]);
@@ -198,7 +202,10 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
     s += (double)near;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) lse[b] = M == -INFINITY ? INFINITY : ((double)C + log2(s)) / (double)kLog2e;
+    if (lane == 0) {
+      largest[b] = M == -INFINITY ? 0.0 : (double)M;
+      log_sum[b] = M == -INFINITY ? INFINITY : log2(s) / (double)kLog2e;
+    }
   }
   __syncthreads();
 
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
         if (i == b * strips) sc = score_of[b];
       } else {
         const float m = stats[(long long)g0 * strips + i].m;
-        if (m > -INFINITY) sc = score_of[b] + ((double)m - lse[b]);
+        if (m > -INFINITY) sc = score_of[b] + (((double)m - largest[b]) - log_sum[b]);
       }
       if (sc > -INFINITY) r.key = order_of(sc);
     }
@@ -309,7 +316,8 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(
     const Ranked c = cand[i];
     if (c.key == 0) continue;
     const int b = (int)(c.at >> 32) - g0;
-    const double sc = done[b] ? score_of[b] : score_of[b] + ((double)value_of((uint32_t)c.key) - lse[b]);
+    const double sc =
+        done[b] ? score_of[b] : score_of[b] + (((double)value_of((uint32_t)c.key) - largest[b]) - log_sum[b]);
     cand_score[i] = sc;
     cand[i].key = order_of(sc);
   }

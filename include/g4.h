@@ -491,7 +491,8 @@ int g4_kv_attend(g4_kv *kv, int layer, const g4_kv_queries *rows, void *work, si
  * (g4_kv_fork's src).  finished_dev (int32, NULL: none): a finished row has one
  * continuation, pad_token at its own score.  Logits of -inf (masked tokens) and
  * NaN are never chosen (a row with a logit of +inf has no continuation); where
- * too few remain: score -inf, parent and token -1.
+ * too few remain: score -inf, parent and token -1.  Every finite logit is a
+ * candidate, the type's lowest among them (a mask of finite values only ranks last).
  * new_scores may be scores.  beams <= 32; work as for g4_kv_attend. */
 size_t g4_beam_select_workspace(int n_rows, int vocab, int beams);
 int g4_beam_select(g4_ctx *ctx, const float *logits_dev, int64_t stride, int vocab, const float *scores_dev,

@@ -1,0 +1,68 @@
+"""Calls of the paged operators that their documentation allows and that are easy
+to get wrong: finite masks, extreme and non-finite values, one-row strides,
+arguments on other streams, refused resizes, freed handles."""
+import numpy as np
+import pytest
+import torch
+
+from tests import paged_ref as ref
+from tests.test_paged_gpu import (EDGES, ROPE_TOL, attend_case, host, i32, mirrored, new_cache, pair_size, same_state,
+                                  select)
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ beam selection
+
+
+def continuations(logits, scores, beams):
+    """paged_ref.beam of rows without -inf, with every log probability taken as
+    (x - max) - log sum exp(x - max): beside a maximum of -1e20 the logarithm
+    would be rounded away."""
+    x = np.asarray(logits, np.float64)
+    x = x - x.max(1, keepdims=True)
+    p = np.asarray(scores, np.float64)[:, None] + (x - np.log(np.exp(x).sum(1, keepdims=True)))
+    out = []
+    for g in range(0, len(x), beams):
+        row, token = np.divmod(np.argsort(-p[g:g + beams].reshape(-1), kind="stable")[:beams], x.shape[1])
+        out.append((p[g + row, token], g + row, token))
+    return [np.concatenate(a) for a in zip(*out)]
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("mask", [-1e6, -3e9, -1e10, -1e11, -1e12, -1e15, -1e20, -1e30, -1e38,
+                                  float(np.finfo(np.float32).min)])
+def test_beam_finite_masks(g4, ctx, mask, offset):
+    """Masks that are very low but finite: pieces of a row without a live token,
+    rows without any, a group with fewer live tokens than beams."""
+    rng = np.random.default_rng(17)
+    beams, vocab = 4, 5003
+    logits = np.full((20, vocab), mask, np.float32)
+    logits[:4, 2100:2110] = rng.standard_normal((4, 10))
+    logits[4:8, [7, 4999]] = rng.standard_normal((4, 2))
+    logits[8, 5] = 1.0       # its group's other rows have nothing live
+    logits[12:16] = mask     # nor has any row of this group
+    logits[16, 3000] = -2.0  # one live token, the other beams do not exist yet
+    scores = -1.5 * rng.permutation(20).astype(np.float32) - 0.25
+    scores[17:] = -np.inf
+    wide = torch.zeros(20, vocab + 5, device="cuda")
+    wide[:, offset:offset + vocab] = torch.from_numpy(logits)
+    new, par, tok = select(g4, ctx, wide[:, offset:offset + vocab], torch.from_numpy(scores).cuda(), beams)
+    want = continuations(logits, scores, beams)
+    assert np.array_equal(host(par), want[1]) and np.array_equal(host(tok), want[2])
+    # as in test_paged_gpu.py: the row's sum to 2^-18, then one rounding
+    assert np.all(abs(host(new) - want[0]) <= 2.0 ** -18 + 2.0 ** -24 * abs(want[0]))
+
+
+def test_beam_extreme_logits(g4, ctx):
+    """The largest finite logits, and both ends of the type in one row."""
+    top = float(np.finfo(np.float32).max)
+    rng = np.random.default_rng(4)
+    logits = np.stack([np.full(3000, top), np.where(rng.random(3000) < 0.5, top, -top),
+                       1e38 * rng.random(3000)]).astype(np.float32)
+    scores = np.array([-1.0, -2.5, -30.0], np.float32)
+    for beams in (1, 3):
+        new, par, tok = select(g4, ctx, torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda(), beams)
+        want = continuations(logits, scores, beams)
+        assert np.array_equal(host(par), want[1]) and np.array_equal(host(tok), want[2])
+        assert np.all(abs(host(new) - want[0]) <= 2.0 ** -18 + 2.0 ** -24 * abs(want[0]))
