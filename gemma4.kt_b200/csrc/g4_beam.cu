@@ -45,17 +45,17 @@ struct StripStat {
   float m, sum;
 };
 
-// A number's order as an unsigned word (NaN below everything).
+// A number's order as an unsigned word (NaN below everything, the zeros equal).
 __device__ __forceinline__ uint32_t order_of(float v) {
   if (!(v == v)) return 0u;
-  const uint32_t u = __float_as_uint(v);
+  const uint32_t u = v == 0.f ? 0u : __float_as_uint(v);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ unsigned long long order_of(double v) {
-  const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+  const unsigned long long u = v == 0.0 ? 0ull : (unsigned long long)__double_as_longlong(v);
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 

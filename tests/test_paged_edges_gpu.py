@@ -66,3 +66,15 @@ def test_beam_extreme_logits(g4, ctx):
         want = continuations(logits, scores, beams)
         assert np.array_equal(host(par), want[1]) and np.array_equal(host(tok), want[2])
         assert np.all(abs(host(new) - want[0]) <= 2.0 ** -18 + 2.0 ** -24 * abs(want[0]))
+
+
+def test_beam_zeros_of_either_sign(g4, ctx):
+    """-0 and +0 are equal: the lower token, the lower beam."""
+    for vocab, low, high in ((40, 3, 30), (3000, 100, 101), (3000, 100, 2500), (3000, 2100, 2101)):
+        logits = np.full((1, vocab), -1.0, np.float32)
+        logits[0, low], logits[0, high] = -0.0, 0.0
+        _, _, tok = select(g4, ctx, torch.from_numpy(logits).cuda(), torch.zeros(1, device="cuda"), 1)
+        assert tok.tolist() == [low]
+    logits = torch.zeros(2, 9, device="cuda")
+    new, par, tok = select(g4, ctx, logits, torch.tensor([-0.0, 0.0], device="cuda"), 2, i32([1, 1]), 4)
+    assert par.tolist() == [0, 1] and tok.tolist() == [4, 4] and new.tolist() == [0.0, 0.0]
