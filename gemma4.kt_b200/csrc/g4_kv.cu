@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
   int* el = en + n;             // shared-page candidate: the last, partly filled page (-1: none)
   int* ec = el + n;             // 1: that page is copied
   int* ea = ec + n;             // first of the entry's pages in free_list
-  __shared__ long long sums64[2][32];
+  __shared__ unsigned long long sums64[2][32];
   __shared__ int sums[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ps = d.page_size;
   grid_dep_launch();
@@ -177,8 +177,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
   }
   // a shared last page is copied by every sequence that grows into it, except
   // one that is left as its only holder; pages wanted per entry
-  // (both sums in one scan: pages in the low, copies in the high half)
-  long long base = 0;
+  // (both sums in one scan: pages in the low 44 bits, since 4096 entries of 2^26
+  // pages and a copy each pass 32 bits but not 39, copies, 4096 at most, above)
+  constexpr int kCopyShift = 44;
+  constexpr unsigned long long kPageMask = (1ull << kCopyShift) - 1;
+  unsigned long long base = 0;
   for (int i0 = 0, round = 0; i0 < n; i0 += kPlanThreads, ++round) {
     const int i = i0 + tid;
     int need = 0, copied = 0;
@@ -194,16 +197,18 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
       const int more = (en[i] + ps - 1) / ps - (eo[i] + ps - 1) / ps;
       need = max(0, more) + copied;
     }
-    long long sum;
-    const long long at = base + block_scan(((long long)copied << 32) | need, sums64[round & 1], &sum);
+    unsigned long long sum;
+    const unsigned long long at =
+        base + block_scan(((unsigned long long)copied << kCopyShift) | (unsigned long long)need, sums64[round & 1], &sum);
     if (i < n) {
-      ea[i] = (int)at;
+      ea[i] = (int)(at & kPageMask);  // (read when all of them have a page: at most n_pages)
       ec[i] = copied;
     }
-    if (copied) moves[at >> 32] = KvMove{el[i], i, eo[i] % ps};  // dst: the entry, its page below
+    if (copied) moves[at >> kCopyShift] = KvMove{el[i], i, eo[i] % ps};  // dst: the entry, its page below
     base += sum;
   }
-  const int total = (int)base, copies = (int)(base >> 32);
+  const long long total = (long long)(base & kPageMask);
+  const int copies = (int)(base >> kCopyShift);
   // the lowest free pages
   int found = 0;
   if (total > 0) {
@@ -234,7 +239,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
     }
     return;
   }
-  for (int k = tid; k < total; k += kPlanThreads) d.refs[free_list[k]] = 1;
+  for (int k = tid; k < (int)total; k += kPlanThreads) d.refs[free_list[k]] = 1;  // (no more than n_pages)
   for (int k = tid; k < copies; k += kPlanThreads) {
     const int i = moves[k].dst;
     moves[k].dst = free_list[ea[i]];

@@ -78,3 +78,28 @@ def test_beam_zeros_of_either_sign(g4, ctx):
     logits = torch.zeros(2, 9, device="cuda")
     new, par, tok = select(g4, ctx, logits, torch.tensor([-0.0, 0.0], device="cuda"), 2, i32([1, 1]), 4)
     assert par.tolist() == [0, 1] and tok.tolist() == [4, 4] and new.tolist() == [0.0, 0.0]
+
+
+# ------------------------------------------------------------------ pages
+
+
+def test_resize_to_more_pages_than_32_bits_count(g4, ctx):
+    """4096 sequences of 2^20 pages each: 2^31 pages wanted, 2^32, and a few around them."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs a page table of 17 GB")
+    n, most = 4096, 1 << 24
+    cache = new_cache(g4, ctx, kv=(1,), hs=(8,), pages=40, seqs=n, positions=most)
+    cache.resize(i32([5, 0]), i32([17, 33]))
+    cache.fork(i32([5, 5]), i32([9, 7]))
+    assert cache.check() == 40 - 5
+    lens, refs, table = cache.lens.clone(), cache.refs.clone(), cache.table[:16, :8].clone()
+    order = torch.arange(n, dtype=torch.int32, device="cuda")
+    for many, longest in ((2048, most), (2047, most), (4096, most), (4095, most), (4096, most // 2)):
+        cache.resize(order[:many], torch.full((many,), longest, dtype=torch.int32, device="cuda"))
+        with pytest.raises(g4.G4Error, match="free pages"):
+            cache.check()
+        assert torch.equal(cache.lens, lens) and torch.equal(cache.refs, refs)
+        assert torch.equal(cache.table[:16, :8], table) and int((cache.table.amax(1) >= 0).sum()) == 4
+    cache.resize(i32([9, 1]), i32([18, 40]))  # one copy, three pages
+    assert cache.check() == 35 - 4
+    del cache
