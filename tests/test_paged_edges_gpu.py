@@ -103,3 +103,31 @@ def test_resize_to_more_pages_than_32_bits_count(g4, ctx):
     cache.resize(i32([9, 1]), i32([18, 40]))  # one copy, three pages
     assert cache.check() == 35 - 4
     del cache
+
+
+@pytest.mark.parametrize("seqs,lens", [
+    ([1, 3, 0, 2], [10, 20, 34, 100]),  # whole pages given back, shared ones among them, then too few
+    ([3, 2, 1], [0, 128, 0]),           # a sequence freed, another, and still too few
+    ([0, 3, 2, 1], [40, 36, 90, 16]),   # a shared last page that both holders want to grow into
+    ([4, 1, 2], [1, 33, 128]),
+])
+def test_refused_resize_restores_the_pages(g4, ctx, seqs, lens):
+    """What a call gives back before it finds too few pages is taken again."""
+    cache = new_cache(g4, ctx, kv=(1, 2), hs=(8, 16), pages=8, seqs=5, positions=128)
+    sim = mirrored(cache)
+    for a in (cache, sim):
+        s = (lambda x: i32(x)) if a is cache else (lambda x: x)
+        a.resize(s([0, 1]), s([33, 40]))
+        a.fork(s([0]), s([3]))
+    same_state(cache, sim)
+    assert cache.check() == 2
+    for _ in range(2):
+        cache.resize(i32(seqs), i32(lens))
+        assert sim.resize(seqs, lens) is False
+        same_state(cache, sim)
+        with pytest.raises(g4.G4Error, match="free pages"):
+            cache.check()
+    cache.resize(i32([1, 3, 2]), i32([0, 35, 50]))  # the same cache goes on
+    assert sim.resize([1, 3, 2], [0, 35, 50])
+    same_state(cache, sim)
+    assert cache.check() == int((sim.refs == 0).sum())
