@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(AttendShape<TYPE, HSP, MT>::kThreads, AttendSh
       for (int i = 1; i < NA; ++i) m = fmaxf(m, q_max[i][lane >> 2]);
       int e = 0;
       if (m > 0.f && m < INFINITY) frexpf(m, &e);
-      e = max(-100, min(100, e - 14));
+      e = max(-126, e - 14);  // (a float's exponent is 128 at most: the factor 2^-e is a normal number at both ends)
       if (warp == 0 && (lane & 3) == 0) q_unscale[lane >> 2] = ldexpf(1.f, e);
       const float f = ldexpf(1.f, -e);
 #pragma unroll

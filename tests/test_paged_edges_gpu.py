@@ -131,3 +131,14 @@ def test_refused_resize_restores_the_pages(g4, ctx, seqs, lens):
     assert sim.resize([1, 3, 2], [0, 35, 50])
     same_state(cache, sim)
     assert cache.check() == int((sim.refs == 0).sum())
+
+
+# ------------------------------------------------------------------ attention
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("power", [122, 119, 100, -99, -95])
+def test_attend_query_ranges(g4, ctx, kind, power):
+    """Queries of any finite size, the scale bringing the scores back."""
+    attend_case(g4, ctx, kind, 64, 1, 8, 16, [(0, 200), (1, 33), (2, 0)], q_size=2.0 ** power, scale=2.0 ** -power,
+                seed=11)
