@@ -142,3 +142,19 @@ def test_attend_query_ranges(g4, ctx, kind, power):
     """Queries of any finite size, the scale bringing the scores back."""
     attend_case(g4, ctx, kind, 64, 1, 8, 16, [(0, 200), (1, 33), (2, 0)], q_size=2.0 ** power, scale=2.0 ** -power,
                 seed=11)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_attend_reports_any_entry_that_is_no_page(g4, ctx, kind):
+    """A visible position whose table entry is no page, whatever it is."""
+    for entry in (-1, -2, -3, -2 ** 31, 16, 2 ** 31 - 1):
+        cache = new_cache(g4, ctx, kind, (1,), (64,), 16, 16, 2, 256)
+        cache.resize(i32([0]), i32([160]))
+        for p in (cache.k(0), cache.v(0)):
+            p.fill_(0.5)
+        cache.table[0, 3] = entry
+        out = torch.empty(1, 128, device="cuda")
+        cache.attend(0, torch.ones(1, 128, device="cuda"), out, i32([0]), i32([150]))
+        with pytest.raises(g4.G4Error, match="without a page"):
+            cache.check()
+        assert torch.all(out == 0.5)
