@@ -263,9 +263,10 @@ int rope_prepare() {
   return e;
 }
 
+// (one row has no distance to the next)
 static bool rows_ok(const void* p, long long stride, int heads, int hs, int n) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 4 == 0 &&
-         (n <= 1 || stride >= (long long)heads * hs);
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 &&
+         (n <= 1 || (stride % 4 == 0 && stride >= (long long)heads * hs));
 }
 
 }  // namespace g4

@@ -158,3 +158,32 @@ def test_attend_reports_any_entry_that_is_no_page(g4, ctx, kind):
         with pytest.raises(g4.G4Error, match="without a page"):
             cache.check()
         assert torch.all(out == 0.5)
+
+
+# ------------------------------------------------------------------ rows
+
+
+def test_one_row_of_a_wider_tensor(g4, ctx):
+    """The distance between rows does not matter where there is one."""
+    hs, heads, kv = 64, 4, 2
+    cache = new_cache(g4, ctx, kv=(kv,), hs=(hs,), pages=4, seqs=2, positions=64)
+    cache.resize(i32([1]), i32([20]))
+    rng = np.random.default_rng(0)
+    wide = torch.from_numpy(rng.standard_normal((3, (heads + 2 * kv) * hs + 1)).astype(np.float32)).cuda()
+    q, k, v = (wide[:1, a * hs:b * hs] for a, b in ((0, heads), (heads, heads + kv), (heads + kv, heads + 2 * kv)))
+    assert q.stride(0) % 4
+    rope = g4.Rope(ctx, hs)
+    out = torch.empty(heads * hs, 1, device="cuda").t()  # [1, heads * hs], one entry "between rows"
+    cache.append(0, q, k, v, out, i32([1]), i32([17]), rope=rope)
+    cache.check()
+    page = int(cache.table[1, 1])
+    f, g = ref.frequencies(hs, 1e4)
+    for got, x, turned in ((out, q, True), (cache.k(0)[page, :, 1], k, True), (cache.v(0)[page, :, 1], v, False)):
+        x = host(x).reshape(1, -1, hs)
+        want = ref.rotate(x, [17], f, g, "half") if turned else x
+        assert np.all(abs(host(got).reshape(x.shape) - want) <= ROPE_TOL * pair_size(want, "half", hs))
+    again = torch.empty_like(out)
+    rope.apply(q, again, i32([17]))
+    assert torch.equal(again, out)
+    with pytest.raises(g4.G4Error, match="aligned"):  # two rows an odd distance apart
+        rope.apply(wide[:2, :hs], torch.empty(2, hs, device="cuda"), i32([1, 2]))
