@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kAppendThreads, NQ == 1 ? 7 : NQ == 2 ? 6 : 4)
       for (int u = 0; u < NQ; ++u) {
         if (lane + 32 * u >= quads) continue;
         float4 v = x[i][u];
-        if (is_q || is_k) {
+        if ((is_q || is_k) && lane + 32 * u < rq) {  // (times 1 and 0 would spread an infinity to its neighbour)
           // pairs (x, z), (y, w) of a split group, (x, y), (z, w) otherwise
           const float b0 = split[u] ? v.z : v.y, a1 = split[u] ? v.y : v.z;
           const float y0 = v.x * cs[u].x - b0 * cs[u].y, z0 = v.x * cs[u].y + b0 * cs[u].x;

@@ -187,3 +187,25 @@ def test_one_row_of_a_wider_tensor(g4, ctx):
     assert torch.equal(again, out)
     with pytest.raises(g4.G4Error, match="aligned"):  # two rows an odd distance apart
         rope.apply(wide[:2, :hs], torch.empty(2, hs, device="cuda"), i32([1, 2]))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_unrotated_elements_stay(g4, ctx, layout):
+    """Elements behind rot_dim, and rows without a rotation, come out as they went
+    in, infinities, NaN and signed zeros among them."""
+    special = torch.tensor([torch.inf, -torch.inf, torch.nan, -0.0, 3e38, 1e-42], device="cuda")
+    x = torch.randn(6, 2 * 96, device="cuda")
+    for i in range(6):
+        x[i, 40 + 7 * i] = special[i]
+        x[i, 96 + 95 - i] = special[5 - i]
+    bits = lambda t: t.contiguous().view(torch.int32)  # noqa: E731
+    out = torch.empty_like(x)
+    g4.Rope(ctx, 96, rot_dim=32, layout=layout).apply(x, out, i32(range(6)))
+    assert torch.equal(bits(out.view(6, 2, 96)[..., 32:]), bits(x.view(6, 2, 96)[..., 32:]))
+    cache = new_cache(g4, ctx, kv=(2,), hs=(96,), pages=4, seqs=1, positions=64)
+    cache.resize(i32([0]), i32([6]))
+    cache.append(0, x, x, x, out, i32([0] * 6), i32(range(6)))  # no rotation at all
+    cache.check()
+    page = int(cache.table[0, 0])
+    for got in (out.view(6, 2, 96), cache.k(0)[page, :, :6].transpose(0, 1), cache.v(0)[page, :, :6].transpose(0, 1)):
+        assert torch.equal(bits(got), bits(x.view(6, 2, 96)))
