@@ -160,6 +160,21 @@ def test_attend_reports_any_entry_that_is_no_page(g4, ctx, kind):
         assert torch.all(out == 0.5)
 
 
+@pytest.mark.parametrize("hs", [64, 80, 256, 512])
+@pytest.mark.parametrize("page", [16, 256])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (7, 1), (64, 4), (100, 70), (1000, 3), (16, 500)])
+def test_attend_windows_of_an_fp32_cache(g4, ctx, hs, page, window, sinks):
+    attend_case(g4, ctx, "f32", hs, 2, 6, page, EDGES + [(11, 999), (12, 640)], window=window, sinks=sinks, seed=hs + window)
+
+
+@pytest.mark.parametrize("kind,hs", [("f32", 64), ("f32", 128), ("f32", 256), ("f32", 512), ("f16", 128), ("bf16", 256)])
+def test_attend_more_rows_than_a_warp_finds(g4, ctx, kind, hs):
+    rng = np.random.default_rng(hs)
+    for n in (128, 129, 301):
+        rows = [(i % 70, int(p)) for i, p in enumerate(rng.permutation(400)[:n] - 2)]
+        attend_case(g4, ctx, kind, hs, 1, 3, 32, rows, window=60, sinks=3, seed=n)
+
+
 # ------------------------------------------------------------------ rows
 
 
@@ -209,3 +224,19 @@ def test_unrotated_elements_stay(g4, ctx, layout):
     page = int(cache.table[0, 0])
     for got in (out.view(6, 2, 96), cache.k(0)[page, :, :6].transpose(0, 1), cache.v(0)[page, :, :6].transpose(0, 1)):
         assert torch.equal(bits(got), bits(x.view(6, 2, 96)))
+
+
+@pytest.mark.parametrize("scaling,attn_factor", [("none", 1.75), ("linear", 0.3), ("yarn", 1.2), ("yarn", -2.0)])
+def test_rope_attn_factor(g4, ctx, scaling, attn_factor):
+    """The factor on cosine and sine instead of the scaling's own."""
+    rng = np.random.default_rng(2)
+    pos = np.array([0, 9, 70000])
+    x = rng.standard_normal((3, 2, 64)).astype(np.float32)
+    kw = {} if scaling == "none" else dict(factor=8.0)
+    out = torch.empty(3, 128, device="cuda")
+    g4.Rope(ctx, 64, rot_dim=48, scaling=scaling, attn_factor=attn_factor, **kw).apply(
+        torch.from_numpy(x.reshape(3, -1)).cuda(), out, i32(pos))
+    f, _ = ref.frequencies(48, 1e4, scaling, **kw)
+    want = ref.rotate(x, pos, f, attn_factor, "half")
+    # one more rounding than ROPE_TOL counts, the factor's, and none of the norm's
+    assert np.all(abs(host(out).reshape(x.shape) - want) <= ROPE_TOL * pair_size(want, "half", 48) + 1e-30)
