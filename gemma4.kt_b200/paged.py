@@ -299,9 +299,11 @@ class KvCache:
         dev, f32, i32, n = self.ctx.device, torch.float32, torch.int32, pos.numel()
         if not 0 <= layer < len(self.head_size):
             raise ValueError(f"layer {layer} of {len(self.head_size)}")
+        if (k is None) is not (v is None) or (q is not None and q_out is None):
+            raise ValueError("k and v go together, and q needs q_out")
         hs, width = self.head_size[layer], self.n_kv_heads[layer] * self.head_size[layer]
         heads = qp = qs = op = os_ = kp = ks = vp = vs = 0
-        if k is not None or v is not None:
+        if k is not None:
             kp, ks = _matrix(dev, k, "k", f32, n, width)
             vp, vs = _matrix(dev, v, "v", f32, n, width)
         if q is not None:

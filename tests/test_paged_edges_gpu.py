@@ -240,3 +240,19 @@ def test_rope_attn_factor(g4, ctx, scaling, attn_factor):
     want = ref.rotate(x, pos, f, attn_factor, "half")
     # one more rounding than ROPE_TOL counts, the factor's, and none of the norm's
     assert np.all(abs(host(out).reshape(x.shape) - want) <= ROPE_TOL * pair_size(want, "half", 48) + 1e-30)
+
+
+# ------------------------------------------------------------------ handles and streams
+
+
+def test_half_given_arguments_are_refused(g4, ctx):
+    cache = new_cache(g4, ctx, kv=(1,), hs=(16,), pages=4, seqs=2, positions=64)
+    cache.resize(i32([0]), i32([20]))
+    x, r = torch.ones(1, 16, device="cuda"), i32([0])
+    for q, k, v, out in ((x, x, None, x), (x, None, x, x), (x, x, x, None), (None, x, None, None), (x, None, None, None)):
+        with pytest.raises(ValueError):
+            cache.append(0, q, k, v, out, r, r)
+    with pytest.raises(g4.G4Error):
+        cache.append(0, None, None, None, None, r, r)
+    cache.check()
+    assert int((cache.k(0) != 0).sum()) == 0
