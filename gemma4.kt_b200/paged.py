@@ -88,6 +88,20 @@ def _matrix(device: int, t, name: str, dtype, rows: int, width: int):
     _wrong(device, t, name, dtype, f"[{rows}, {width}] with consecutive columns")
 
 
+def _open(ctx: Context, what: str) -> None:
+    if not ctx.handle:
+        raise ValueError(f"{what}: the context is closed")
+
+
+def _failed(rc: int, ctx: Context, handle, what: str) -> None:
+    """Raises what a call's status says; a handle that was freed, or whose context
+    is closed, reaches the library as NULL."""
+    _open(ctx, what)
+    if not handle:
+        raise ValueError(f"{what}: it was freed")
+    check(rc, ctx.handle, what)
+
+
 class _Owner:
     """Frees a handle when the last object that uses its memory is gone."""
 
@@ -122,6 +136,7 @@ class Rope:
     def __init__(self, ctx: Context, head_size: int, rot_dim: int | None = None, theta: float = 10000.0,
                  layout: str = "half", scaling: str = "none", factor: float = 1.0, original_ctx: int = 4096,
                  beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0, freq_factors=None):
+        _open(ctx, "Rope")
         if layout not in _LAYOUTS or scaling not in _SCALINGS:
             raise ValueError(f"layout {layout!r} (half, interleaved), scaling {scaling!r} (none, linear, yarn)")
         rot_dim = head_size if rot_dim is None else rot_dim
@@ -155,9 +170,10 @@ class Rope:
         xp, xs = _matrix(dev, x, "x", torch.float32, rows, width)
         op, os_ = _matrix(dev, out, "out", torch.float32, rows, width)
         pp = _vector(dev, pos, "pos", torch.int32, rows)
-        rc = self._apply(self.handle, xp, xs, op, os_, width // self.head_size, pp, rows, _stream(dev, stream))
+        rc = self._apply(self.handle if self.ctx.handle else None, xp, xs, op, os_, width // self.head_size, pp, rows,
+                         _stream(dev, stream))
         if rc:
-            check(rc, self.ctx.handle, "g4_rope_apply")
+            _failed(rc, self.ctx, self.handle, "g4_rope_apply")
 
 
 class KvCache:
@@ -166,6 +182,7 @@ class KvCache:
 
     def __init__(self, ctx: Context, n_kv_heads, head_size, dtype=GGMLType.BF16, page_size: int = 32,
                  n_pages: int = 1024, n_seqs: int = 64, max_positions: int = 4096):
+        _open(ctx, "KvCache")
         heads, sizes = np.array(n_kv_heads, np.int32), np.array(head_size, np.int32)
         if heads.ndim != 1 or heads.shape != sizes.shape or not heads.size:
             raise ValueError("n_kv_heads and head_size must list the same layers")
@@ -255,9 +272,9 @@ class KvCache:
         dev, n = self.ctx.device, a.numel()
         ap = _vector(dev, a, names[0], torch.int32, n)
         bp = _vector(dev, b, names[1], torch.int32, n)
-        rc = fn(self.handle, ap, bp, n, _stream(dev, stream))
+        rc = fn(self.handle if self.ctx.handle else None, ap, bp, n, _stream(dev, stream))
         if rc:
-            check(rc, self.ctx.handle, fn.__name__)
+            _failed(rc, self.ctx, self.handle, fn.__name__)
 
     def resize(self, seqs, lens, stream=None) -> None:
         """Pages for lens[i] positions of sequence seqs[i] (int32 tensors; 0 frees
@@ -276,14 +293,17 @@ class KvCache:
 
     def compact(self, stream=None) -> None:
         """Live pages to the front of the pool; the table follows."""
-        check(self._lib.g4_kv_compact(self.handle, _stream(self.ctx.device, stream)), self.ctx.handle, "g4_kv_compact")
+        rc = self._lib.g4_kv_compact(self.handle if self.ctx.handle else None, _stream(self.ctx.device, stream))
+        if rc:
+            _failed(rc, self.ctx, self.handle, "g4_kv_compact")
 
     def check(self, stream=None) -> int:
         """Wait for the stream; raise what the cache's calls recorded, else the
         number of free pages."""
         n = C.c_int()
-        check(self._lib.g4_kv_check(self.handle, C.byref(n), _stream(self.ctx.device, stream)), self.ctx.handle,
-              "g4_kv_check")
+        rc = self._lib.g4_kv_check(self.handle if self.ctx.handle else None, C.byref(n), _stream(self.ctx.device, stream))
+        if rc:
+            _failed(rc, self.ctx, self.handle, "g4_kv_check")
         return n.value
 
     # ---- rows
@@ -317,10 +337,14 @@ class KvCache:
                           _vector(dev, pos, "pos", i32, n),
                           0 if q_norm is None else _vector(dev, q_norm, "q_norm", f32, hs),
                           0 if k_norm is None else _vector(dev, k_norm, "k_norm", f32, hs), bool(v_norm), eps)
-        rc = self._lib.g4_kv_append(self.handle, layer, rows, None if rope is None else rope.handle,
-                                    _stream(dev, stream))
+        turns = None
+        if rope is not None:
+            turns = rope.handle
+            if not turns:  # NULL would store the rows without a rotation
+                raise ValueError("the rotary plan was freed")
+        rc = self._lib.g4_kv_append(self.handle if self.ctx.handle else None, layer, rows, turns, _stream(dev, stream))
         if rc:
-            check(rc, self.ctx.handle, "g4_kv_append")
+            _failed(rc, self.ctx, self.handle, "g4_kv_append")
 
     def attend(self, layer: int, q, out, seqs, pos, scale: float = 1.0, window: int = 0, sinks: int = 0,
                stream=None) -> None:
@@ -342,9 +366,10 @@ class KvCache:
         rows = _QUERIES.pack(n, heads, qp, op, qs, os_, _vector(dev, seqs, "seqs", i32, n),
                              _vector(dev, pos, "pos", i32, n), scale, window, sinks)
         work = _workspace(self.ctx, self._work[layer], stream)
-        rc = self._lib.g4_kv_attend(self.handle, layer, rows, work.data_ptr(), self._work[layer], _stream(dev, stream))
+        rc = self._lib.g4_kv_attend(self.handle if self.ctx.handle else None, layer, rows, work.data_ptr(),
+                                    self._work[layer], _stream(dev, stream))
         if rc:
-            check(rc, self.ctx.handle, "g4_kv_attend")
+            _failed(rc, self.ctx, self.handle, "g4_kv_attend")
 
 
 def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, tokens, finished=None,
@@ -370,4 +395,4 @@ def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, t
     rc = L.g4_beam_select(ctx.handle, lp, ls, vocab, sp, fp, rows, beams, pad_token, np_, pp, tp, work.data_ptr(),
                           work.numel(), _stream(dev, stream))
     if rc:
-        check(rc, ctx.handle, "g4_beam_select")
+        _failed(rc, ctx, ctx.handle, "g4_beam_select")

@@ -256,3 +256,37 @@ def test_half_given_arguments_are_refused(g4, ctx):
         cache.append(0, None, None, None, None, r, r)
     cache.check()
     assert int((cache.k(0) != 0).sum()) == 0
+
+
+def test_freed_handles_are_refused(g4, ctx):
+    cache = new_cache(g4, ctx, kv=(1,), hs=(16,), pages=4, seqs=2, positions=64)
+    cache.resize(i32([0]), i32([20]))
+    rope = g4.Rope(ctx, 16)
+    x, r = torch.ones(1, 16, device="cuda"), i32([0])
+    out = torch.full_like(x, 9.0)
+    rope.free()
+    with pytest.raises(ValueError, match="freed"):  # and not stored without a rotation
+        cache.append(0, x, x, x, out, r, r, rope=rope)
+    with pytest.raises(ValueError, match="freed"):
+        rope.apply(x, out, r)
+    cache.check()
+    assert torch.all(out == 9.0) and int((cache.k(0) != 0).sum()) == 0
+    cache.free()
+    for call in (lambda: cache.append(0, x, x, x, out, r, r), lambda: cache.attend(0, x, out, r, r),
+                 lambda: cache.resize(r, r), lambda: cache.fork(r, r), lambda: cache.copy_pages(r, r), cache.compact,
+                 cache.check, lambda: cache.table, lambda: cache.k(0)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_calls_after_the_context_are_refused(g4):
+    c = g4.Context(0)
+    cache, rope = new_cache(g4, c, kv=(1,), hs=(16,), pages=4), g4.Rope(c, 16)
+    x, r = torch.ones(1, 16, device="cuda"), i32([0])
+    c.close()
+    for call in (lambda: cache.append(0, x, x, x, x, r, r), lambda: cache.attend(0, x, x, r, r),
+                 lambda: cache.resize(r, r), lambda: cache.fork(r, r), lambda: cache.copy_pages(r, r), cache.compact,
+                 cache.check, lambda: rope.apply(x, x, r), lambda: g4.Rope(c, 16), lambda: new_cache(g4, c),
+                 lambda: g4.beam_select(c, x, x[:, 0], 1, x[:, 0], r, r)):
+        with pytest.raises(ValueError, match="closed"):
+            call()
