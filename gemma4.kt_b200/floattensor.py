@@ -14,6 +14,7 @@ UnsupportedOperation, IllegalArgumentException -> ValueError.
 from __future__ import annotations
 
 import ctypes as C
+from collections import deque
 from enum import IntEnum
 
 import numpy as np
@@ -105,9 +106,13 @@ class Context:
         self.handle = h
         self.device = device
         self.work = {}  # work space of the paged operators, by stream
+        self.held = deque()  # what their calls on named streams use: (event behind the call, tensors)
 
     def close(self) -> None:
         self.work = {}
+        for passed, _ in self.held:
+            passed.synchronize()
+        self.held.clear()
         if self.handle:
             lib().g4_destroy(self.handle)
             self.handle = None

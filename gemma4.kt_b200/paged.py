@@ -12,8 +12,12 @@ these are the operators a server or a beam search needs next to the decoder:
     beam_select(ctx, logits, ...)      the next beams, parents for fork
 
 Tensors are torch CUDA tensors on the context's device; every call is
-asynchronous on `stream` (default: torch's current stream of that device) and
-may be captured into a CUDA graph.  What a call finds wrong in device data is
+asynchronous on `stream` (a cudaStream_t as a number; default: torch's current
+stream of that device) and may be captured into a CUDA graph.  A named stream is
+ordered behind what made the tensors by the caller; they may be dropped as soon
+as the call returns.  As everywhere in this package one host thread at a time
+uses a context and what was made from it: its calls on a stream share a work
+space.  What a call finds wrong in device data is
 skipped and reported by KvCache.check().
 """
 from __future__ import annotations
@@ -61,6 +65,33 @@ def _workspace(ctx: Context, n: int, stream):
         return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
     with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=ctx.device)):
         return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", ctx.device))
+
+
+def _release(ctx: Context) -> None:
+    """Lets go of what _hold keeps for calls that their streams have passed."""
+    import torch
+
+    if not torch._C._cuda_isCurrentStreamCapturing():  # (a capture forbids the query)
+        while ctx.held and ctx.held[0][0].query():
+            ctx.held.popleft()
+
+
+def _hold(ctx: Context, stream, *tensors) -> None:
+    """Keeps the tensors that a call on a named stream uses until that stream has
+    passed the call (seen at the next such call or check), so that torch hands
+    their memory to nobody before, even if the caller drops them now.
+    Tensor.record_stream would not do: it touches the stream again when the tensor
+    dies, which may be after the stream (a freed batch's) has gone.  What a graph
+    captures its owner keeps."""
+    import torch
+
+    _release(ctx)
+    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=ctx.device)):
+        if torch._C._cuda_isCurrentStreamCapturing():
+            return
+        passed = torch.cuda.Event()
+        passed.record()
+    ctx.held.append((passed, tensors))
 
 
 def _wrong(device: int, t, name: str, dtype, what: str):
@@ -174,6 +205,8 @@ class Rope:
                          _stream(dev, stream))
         if rc:
             _failed(rc, self.ctx, self.handle, "g4_rope_apply")
+        if stream is not None:
+            _hold(self.ctx, stream, x, out, pos)
 
 
 class KvCache:
@@ -275,6 +308,8 @@ class KvCache:
         rc = fn(self.handle if self.ctx.handle else None, ap, bp, n, _stream(dev, stream))
         if rc:
             _failed(rc, self.ctx, self.handle, fn.__name__)
+        if stream is not None:
+            _hold(self.ctx, stream, a, b)
 
     def resize(self, seqs, lens, stream=None) -> None:
         """Pages for lens[i] positions of sequence seqs[i] (int32 tensors; 0 frees
@@ -302,6 +337,8 @@ class KvCache:
         number of free pages."""
         n = C.c_int()
         rc = self._lib.g4_kv_check(self.handle if self.ctx.handle else None, C.byref(n), _stream(self.ctx.device, stream))
+        if self.ctx.held:
+            _release(self.ctx)
         if rc:
             _failed(rc, self.ctx, self.handle, "g4_kv_check")
         return n.value
@@ -345,6 +382,8 @@ class KvCache:
         rc = self._lib.g4_kv_append(self.handle if self.ctx.handle else None, layer, rows, turns, _stream(dev, stream))
         if rc:
             _failed(rc, self.ctx, self.handle, "g4_kv_append")
+        if stream is not None:
+            _hold(self.ctx, stream, q, k, v, q_out, seqs, pos, q_norm, k_norm)
 
     def attend(self, layer: int, q, out, seqs, pos, scale: float = 1.0, window: int = 0, sinks: int = 0,
                stream=None) -> None:
@@ -370,6 +409,8 @@ class KvCache:
                                     self._work[layer], _stream(dev, stream))
         if rc:
             _failed(rc, self.ctx, self.handle, "g4_kv_attend")
+        if stream is not None:
+            _hold(self.ctx, stream, q, out, seqs, pos)
 
 
 def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, tokens, finished=None,
@@ -396,3 +437,5 @@ def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, t
                           work.numel(), _stream(dev, stream))
     if rc:
         _failed(rc, ctx, ctx.handle, "g4_beam_select")
+    if stream is not None:
+        _hold(ctx, stream, logits, scores, new_scores, parents, tokens, finished)

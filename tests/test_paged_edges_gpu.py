@@ -290,3 +290,91 @@ def test_calls_after_the_context_are_refused(g4):
                  lambda: g4.beam_select(c, x, x[:, 0], 1, x[:, 0], r, r)):
         with pytest.raises(ValueError, match="closed"):
             call()
+
+
+def test_arguments_freed_before_their_stream_ran(g4, ctx):
+    """A call on a named stream keeps its tensors' memory from being handed out
+    again until the stream has used it."""
+    cache = new_cache(g4, ctx, kv=(1,), hs=(16,), pages=64, seqs=8, positions=64)
+    rope = g4.Rope(ctx, 16)
+    for p in (cache.k(0), cache.v(0)):
+        p.copy_(torch.randn(p.shape, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda"))
+    cache.resize(i32([2]), i32([40]))
+    x = torch.randn(4, 16, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    logits, scores = torch.randn(2, 600, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda"), None
+    want, turned, scores = torch.empty_like(x), torch.empty_like(x), torch.zeros(2, device="cuda")
+    cache.attend(0, x, want, i32([2] * 4), i32([3, 39, 0, 20]))
+    rope.apply(x, turned, i32([5, 6, 7, 8]))
+    chosen = select(g4, ctx, logits, scores, 2)
+    out, out2 = torch.empty_like(x), torch.empty_like(x)
+    best = [torch.empty_like(t) for t in chosen]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(300_000_000)  # bounded: about 0.15 s
+    at = side.cuda_stream
+    cache.resize(i32([0, 1]), i32([20, 33]), stream=at)
+    junk = [i32([5, 6]) for _ in range(4)]
+    cache.fork(i32([0, 1]), i32([3, 4]), stream=at)
+    junk += [i32([7, 7]) for _ in range(4)]
+    cache.attend(0, x.clone(), out, i32([2] * 4), i32([3, 39, 0, 20]), stream=at)
+    junk += [torch.zeros_like(x), i32([7] * 4), i32([1] * 4)] * 2
+    rope.apply(x.clone(), out2, i32([5, 6, 7, 8]), stream=at)
+    junk += [torch.zeros_like(x), i32([0] * 4)] * 2
+    g4.beam_select(ctx, logits.clone(), scores.clone(), 2, *best, stream=at)
+    junk += [torch.zeros_like(logits), torch.ones_like(scores)] * 2
+    torch.cuda.synchronize()
+    assert cache.lens.tolist() == [20, 33, 40, 20, 33, 0, 0, 0]
+    assert torch.equal(out, want) and torch.equal(out2, turned)
+    assert all(torch.equal(a, b) for a, b in zip(best, chosen))
+    assert len(ctx.held) >= 5
+    assert cache.check() == 64 - 3 - 2 - 3
+    assert not ctx.held
+
+
+def test_arguments_outlive_their_stream(g4, ctx):
+    """Tensors used on a batch's stream die after the batch."""
+    from tests.test_decode_gpu import SPECS, _models
+
+    _, _, model, _ = _models(g4, ctx, SPECS["q8-gqa8"], seed=21)
+    batch = model.new_paged_batch(2, 32, page_size=16)
+    seqs, lens = i32([0]), i32([20])
+    batch.cache.resize(seqs, lens, stream=batch.stream)
+    batch.free()
+    model.free()
+    del seqs, lens
+    more = [i32([k]) for k in range(8)]
+    torch.cuda.synchronize()
+    assert [int(t) for t in more] == list(range(8))
+
+
+def test_streams_by_number(g4, ctx):
+    """The default stream by its number, and a stream that is being captured."""
+    cache = new_cache(g4, ctx, "bf16", (2,), (128,), 16, 400, 4, 1600)
+    cache.resize(i32(range(4)), i32([1600] * 4))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for p in (cache.k(0), cache.v(0)):
+        p.copy_(torch.randn(p.shape, generator=g, device="cuda"))
+    q, rows, pos = torch.randn(4, 1024, generator=g, device="cuda"), i32(range(4)), i32([1599, 700, 3, 1000])
+    want, out = torch.empty_like(q), torch.zeros_like(q)
+    cache.attend(0, q, want, rows, pos, scale=0.05)
+    torch.cuda.synchronize()
+    cache.attend(0, q, out, rows, pos, scale=0.05, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    out.zero_()
+    logits, scores = torch.randn(4, 5000, generator=g, device="cuda"), torch.zeros(4, device="cuda")
+    chosen = select(g4, ctx, logits, scores, 2)
+    best = [torch.empty_like(t) for t in chosen]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        at = torch.cuda.current_stream().cuda_stream
+        cache.attend(0, q, out, rows, pos, scale=0.05, stream=at)
+        g4.beam_select(ctx, logits, scores, 2, *best, stream=at)
+    for _ in range(3):
+        other = [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(8)]  # memory that the graph must not share
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(best, chosen))
+        assert all(float(t.sum()) == 7.0 * t.numel() for t in other)
+        out.zero_()
