@@ -378,6 +378,9 @@ class PagedBatch(DecoderBatch):
         ctx, vocab = self.model.ctx, self.model.cfg.vocab
         dev = torch.device("cuda", ctx.device)
         with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=dev)):
+            if self.cache.lens[:beams].any():
+                raise ValueError(f"slots 0..{beams - 1} must be free (cache.resize to 0): they hold "
+                                 f"{self.cache.lens[:beams].tolist()} positions")
             last = torch.as_tensor(_DeviceArray(_Owner(None, None), lib().g4_batch_logits(self.handle),
                                                 (self.n_max, vocab), "<f4"), device=dev)
             rows = torch.arange(beams, dtype=torch.int32, device=dev)

@@ -378,3 +378,26 @@ def test_streams_by_number(g4, ctx):
         assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(best, chosen))
         assert all(float(t.sum()) == 7.0 * t.numel() for t in other)
         out.zero_()
+
+
+def test_beam_search_in_occupied_slots_is_refused(g4, ctx):
+    """A slot that holds a sequence is not searched over, and keeps it."""
+    from tests.test_decode_gpu import SPECS, _models
+
+    m, _, model, _ = _models(g4, ctx, SPECS["q8-gqa8"], seed=21)
+    batch = model.new_paged_batch(6, 64, page_size=16)
+    prompt = np.concatenate([[2], m.prompt(20, seed=3)]).astype(np.int32)
+    want, _ = batch.beam_search(prompt, 3, 4)
+    for p, t in enumerate((2, 9, 11)):
+        kept, _ = batch.step([t], [p], slots=[1])
+    lens = batch.cache.lens.clone()
+    with pytest.raises(ValueError, match="slot"):
+        batch.beam_search(prompt, 3, 4)
+    assert torch.equal(batch.cache.lens, lens)
+    again, _ = batch.step([11], [2], slots=[1])  # its last position once more
+    assert np.array_equal(again, kept)
+    batch.cache.resize(i32([1]), i32([0]), stream=batch.stream)
+    got, _ = batch.beam_search(prompt, 3, 4)
+    assert np.array_equal(got, want)
+    batch.free()
+    model.free()
