@@ -336,8 +336,9 @@ class PagedBatch(DecoderBatch):
 
     def __init__(self, model: DecoderModel, n_max: int, max_positions: int, page_size: int = 32,
                  n_pages: int | None = None, dtype=GGMLType.F32):
-        from .paged import KvCache
+        from .paged import KvCache, _int32
 
+        _int32(n_max=n_max, max_positions=max_positions, page_size=page_size, n_pages=n_pages or 0)
         self.page_size, self.dtype = int(page_size), GGMLType(int(dtype))
         self.n_pages = int(n_pages) if n_pages is not None else int(n_max) * -(-int(max_positions) // max(1, self.page_size))
         super().__init__(model, n_max, max_positions)

@@ -119,6 +119,13 @@ def _matrix(device: int, t, name: str, dtype, rows: int, width: int):
     _wrong(device, t, name, dtype, f"[{rows}, {width}] with consecutive columns")
 
 
+def _int32(**values) -> None:
+    """Refuses what a C int does not hold: ctypes would pass its low bits on."""
+    for name, v in values.items():
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{name} {v} is beyond 32 bits")
+
+
 def _open(ctx: Context, what: str) -> None:
     if not ctx.handle:
         raise ValueError(f"{what}: the context is closed")
@@ -168,6 +175,7 @@ class Rope:
                  layout: str = "half", scaling: str = "none", factor: float = 1.0, original_ctx: int = 4096,
                  beta_fast: float = 32.0, beta_slow: float = 1.0, attn_factor: float = 0.0, freq_factors=None):
         _open(ctx, "Rope")
+        _int32(head_size=head_size, rot_dim=0 if rot_dim is None else rot_dim, original_ctx=original_ctx)
         if layout not in _LAYOUTS or scaling not in _SCALINGS:
             raise ValueError(f"layout {layout!r} (half, interleaved), scaling {scaling!r} (none, linear, yarn)")
         rot_dim = head_size if rot_dim is None else rot_dim
@@ -216,6 +224,7 @@ class KvCache:
     def __init__(self, ctx: Context, n_kv_heads, head_size, dtype=GGMLType.BF16, page_size: int = 32,
                  n_pages: int = 1024, n_seqs: int = 64, max_positions: int = 4096):
         _open(ctx, "KvCache")
+        _int32(page_size=page_size, n_pages=n_pages, n_seqs=n_seqs, max_positions=max_positions)
         heads, sizes = np.array(n_kv_heads, np.int32), np.array(head_size, np.int32)
         if heads.ndim != 1 or heads.shape != sizes.shape or not heads.size:
             raise ValueError("n_kv_heads and head_size must list the same layers")
@@ -425,6 +434,7 @@ def beam_select(ctx: Context, logits, scores, beams: int, new_scores, parents, t
         raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
     dev, f32, i32 = ctx.device, torch.float32, torch.int32
     rows, vocab = logits.shape
+    _int32(vocab=vocab, beams=beams, pad_token=pad_token)
     L = lib()
     lp, ls = _matrix(dev, logits, "logits", f32, rows, vocab)
     sp = _vector(dev, scores, "scores", f32, rows)

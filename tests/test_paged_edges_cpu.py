@@ -20,3 +20,30 @@ def test_half_given_arguments(cache):
     for q, k, v, out in ((x, x, None, x), (x, None, x, x), (x, x, x, None), (None, None, x, None), (x, None, None, None)):
         with pytest.raises(ValueError, match="together"):
             cache.append(0, q, k, v, out, r, r)
+
+
+@pytest.mark.parametrize("name", ["page_size", "n_pages", "n_seqs", "max_positions"])
+@pytest.mark.parametrize("excess", [2 ** 32, -2 ** 32, 2 ** 31])
+def test_sizes_beyond_32_bits(g4, cache, name, excess):
+    """A size is not cut to its low 32 bits (the cache's views would reach past its memory)."""
+    good = dict(page_size=16, n_pages=5, n_seqs=2, max_positions=64)
+    good[name] += excess
+    with pytest.raises(ValueError, match=name):
+        g4.KvCache(cache.ctx, [1], [8], **good)
+
+
+def test_other_numbers_beyond_32_bits(g4, cache):
+    x, r = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
+    for kw in (dict(head_size=2 ** 32 + 64), dict(head_size=64, rot_dim=2 ** 32 + 32),
+               dict(head_size=64, scaling="yarn", original_ctx=2 ** 32 + 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            g4.Rope(cache.ctx, **kw)
+    with pytest.raises(ValueError, match="beams"):
+        g4.beam_select(cache.ctx, x, x[:, 0], 2 ** 32 + 2, x[:, 0], r, r)
+    with pytest.raises(ValueError, match="pad_token"):
+        g4.beam_select(cache.ctx, x, x[:, 0], 2, x[:, 0], r, r, pad_token=2 ** 32)
+    model = g4.DecoderModel.__new__(g4.DecoderModel)
+    for kw in (dict(n_max=2 ** 32 + 1), dict(max_positions=2 ** 32 + 64), dict(page_size=2 ** 32 + 16),
+               dict(n_pages=2 ** 32 + 4)):
+        with pytest.raises(ValueError, match="32 bits"):
+            model.new_paged_batch(**{**dict(n_max=2, max_positions=64), **kw})
