@@ -406,12 +406,17 @@ __global__ void __launch_bounds__(kCopyThreads) kv_copy_kernel(KvDev d, const Kv
   }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) kv_count_free_kernel(KvDev d) {
+// g4_kv_check: the number of free pages, and the record, which starts anew.
+__global__ void __launch_bounds__(kPlanThreads) kv_check_kernel(KvDev d) {
   __shared__ int sums[32];
   int mine = 0, sum;
   for (int p = threadIdx.x; p < d.n_pages; p += kPlanThreads) mine += d.refs[p] <= 0;
   block_scan(mine, sums, &sum);
-  if (threadIdx.x == 0) d.flags[1] = (unsigned)sum;
+  if (threadIdx.x == 0) {
+    d.flags[1] = (unsigned)sum;
+    // read and cleared at once: attention on another stream may be recording
+    d.flags[2] = atomicExch(d.flags, 0u);
+  }
 }
 
 static int copy_grid(const g4_kv* kv, long long max_moves) {
@@ -577,7 +582,7 @@ int g4_kv_create(g4_ctx* c, const g4_kv_config* cfg, g4_kv** out) {
   cudaFuncAttributes fa;  // loads the kernels, so that a first call may be captured
   if (!e) e = cudaFuncGetAttributes(&fa, kv_compact_kernel);
   if (!e) e = cudaFuncGetAttributes(&fa, kv_copy_kernel);
-  if (!e) e = cudaFuncGetAttributes(&fa, kv_count_free_kernel);
+  if (!e) e = cudaFuncGetAttributes(&fa, kv_check_kernel);
   if (!e) e = (cudaError_t)rope_prepare();
   if (!e) e = (cudaError_t)kv_attend_prepare(kv);
   if (!e) e = cudaDeviceSynchronize();
@@ -668,21 +673,21 @@ int g4_kv_check(g4_kv* kv, int* free_pages, void* stream) {
     c->set_err("g4_kv_check: waits for the stream, which is being captured");
     return G4_E_ARG;
   }
-  unsigned h[2] = {0, 0};
-  kv_count_free_kernel<<<1, kPlanThreads, 0, st>>>(kv_dev(kv));
+  unsigned read[2] = {0, 0};
+  kv_check_kernel<<<1, kPlanThreads, 0, st>>>(kv_dev(kv));
   e = cudaGetLastError();
-  if (!e) e = cudaMemcpyAsync(h, kv->flags, sizeof h, cudaMemcpyDeviceToHost, st);
-  if (!e) e = cudaMemsetAsync(kv->flags, 0, sizeof(unsigned), st);
+  if (!e) e = cudaMemcpyAsync(read, kv->flags + 1, sizeof read, cudaMemcpyDeviceToHost, st);
   if (!e) e = cudaStreamSynchronize(st);
   if (e) return c->cuda_fail(e, "g4_kv_check");
-  if (free_pages) *free_pages = (int)h[1];
-  if (!h[0]) return 0;
-  c->set_err("g4_kv_check:%s%s%s%s%s", h[0] & KV_NO_PAGES ? " not enough free pages (the resize changed nothing);" : "",
-             h[0] & KV_BAD_ENTRY ? " an entry's sequence, length or page is out of range or named twice;" : "",
-             h[0] & KV_NOT_STORED ? " an appended position has no page or lies in a shared one;" : "",
-             h[0] & KV_BAD_ROW ? " a row's sequence or position is out of range or sees a position without a page;" : "",
-             h[0] & KV_TIMEOUT ? " a bounded wait expired inside a kernel;" : "");
-  return h[0] & KV_NO_PAGES ? G4_E_NOMEM : G4_E_DEVICE;
+  const unsigned found = read[1];
+  if (free_pages) *free_pages = (int)read[0];
+  if (!found) return 0;
+  c->set_err("g4_kv_check:%s%s%s%s%s", found & KV_NO_PAGES ? " not enough free pages (the resize changed nothing);" : "",
+             found & KV_BAD_ENTRY ? " an entry's sequence, length or page is out of range or named twice;" : "",
+             found & KV_NOT_STORED ? " an appended position has no page or lies in a shared one;" : "",
+             found & KV_BAD_ROW ? " a row's sequence or position is out of range or sees a position without a page;" : "",
+             found & KV_TIMEOUT ? " a bounded wait expired inside a kernel;" : "");
+  return found & KV_NO_PAGES ? G4_E_NOMEM : G4_E_DEVICE;
 }
 
 }  // extern "C"

@@ -46,7 +46,7 @@ struct g4_kv {
   uint8_t* pool = nullptr;
   uint8_t* meta = nullptr;     // everything below, one allocation
   int32_t *table = nullptr, *lens = nullptr, *refs = nullptr;
-  unsigned* flags = nullptr;   // [0] status bits, [1] free pages (g4_kv_check)
+  unsigned* flags = nullptr;   // [0] status bits; g4_kv_check leaves free pages in [1] and the bits it took in [2]
   KvStrip* strips = nullptr;   // [n_strips]
   // work space of the calls that change the cache (ordered by the caller)
   int32_t* free_list = nullptr;  // [n_pages] free pages a call takes / the new id of every moved page

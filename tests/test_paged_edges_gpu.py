@@ -380,6 +380,30 @@ def test_streams_by_number(g4, ctx):
         out.zero_()
 
 
+def test_no_report_is_lost_to_a_check_on_another_stream(g4, ctx):
+    """Attention on one stream records a bad row around the moment when a check on
+    another reads and clears the record: one of the checks reports it."""
+    cache = new_cache(g4, ctx, kv=(1,), hs=(16,), pages=4, seqs=2, positions=64)
+    q, out, seqs, pos = torch.ones(1, 16, device="cuda"), torch.empty(1, 16, device="cuda"), i32([0]), i32([5])
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def reports(stream):
+        try:
+            cache.check(stream=stream.cuda_stream)
+        except g4.G4Error:
+            return 1
+        return 0
+
+    torch.cuda.synchronize()
+    for i in range(600):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2500 * (i % 60))
+            cache.attend(0, q, out, seqs, pos)  # a visible position without a page
+        seen = reports(other)
+        side.synchronize()
+        assert seen + reports(other) >= 1, i
+
+
 def test_beam_search_in_occupied_slots_is_refused(g4, ctx):
     """A slot that holds a sequence is not searched over, and keeps it."""
     from tests.test_decode_gpu import SPECS, _models
