@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
     if (copied) moves[at >> kCopyShift] = KvMove{el[i], i, eo[i] % ps};  // dst: the entry, its page below
     base += sum;
   }
-  const long long total = (long long)(base & kPageMask);
+  const int total = (int)min(base & kPageMask, 0x7fffffffull);  // (there are 2^20 pages at most)
   const int copies = (int)(base >> kCopyShift);
   // the lowest free pages
   int found = 0;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_resize_kernel(KvDev d, const 
     }
     return;
   }
-  for (int k = tid; k < (int)total; k += kPlanThreads) d.refs[free_list[k]] = 1;  // (no more than n_pages)
+  for (int k = tid; k < total; k += kPlanThreads) d.refs[free_list[k]] = 1;
   for (int k = tid; k < copies; k += kPlanThreads) {
     const int i = moves[k].dst;
     moves[k].dst = free_list[ea[i]];
