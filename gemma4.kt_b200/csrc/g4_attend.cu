@@ -17,8 +17,11 @@
 // q scaled by a power of two per head so that both parts stay normal); K and V
 // enter the mma exactly.  The tensor core cuts its sums off: they are taken
 // fresh every few steps and added in fp32 (without: 1e-6 to 3e-6 of the result
-// off, growing with the context; with: 2e-7 to 5e-7, less than fp32 matrix
-// products).  An fp32 cache is multiplied in fp32, two products an instruction:
+// off, growing with the context; with: 2e-7 to 6e-7, less than fp32 matrix
+// products). Weights are 32-bit powers of two by the hardware's ex2 (2^-22), their
+// sums 32-bit, where the contiguous batch takes exponentials in 64 bits: one per
+// position and head, which the products would wait for, and an error below what
+// the products leave.  An fp32 cache is multiplied in fp32, two products an instruction:
 // K and V split into parts as well would need six mma steps for one (64
 // sequences to 4000, 8 heads over one of 256: 106 us against 83).
 //
@@ -30,11 +33,11 @@
 // positions change.  Runs that end inside an item leave (max, sum, O) partials
 // in the caller's work space; a second launch joins them in a fixed order.
 //
-// Bound where: 96 ragged sequences to 12001 (64 heads over 8 of 128, bf16) run
-// at the measured copy rate (353 us for 2.37 GB), one of 131071 (f16) at 90% of
-// it; 64 sequences with a window of 512 (16 heads over 8 of 256, bf16) at 73%:
-// what is left is the start of a run (position, page, first bytes: 4 us) and
-// the join (3 us). A call of a few positions takes 8 to 13 us.
+// Bound where (time of the GPU alone): 96 ragged sequences to 12001 (64 heads over
+// 8 of 128, bf16) run at the measured copy rate (360 us for 2.37 GB), one of 131071
+// (f16) at 91% of it (90 us); 64 sequences with a window of 512 (16 heads over 8 of
+// 256, bf16) at 73% (51 us): what is left is the start of a run (position, page,
+// first bytes: 4 us) and the join (3 us). A call of a few positions takes 9 to 14.
 //
 // Inside a run one warp brings units in (TMA boxes of 16 positions x 128 bytes
 // of a head, swizzled so that fragment loads hit distinct banks; K and V of a

@@ -4,18 +4,24 @@
 // One pass over the logits, bound by HBM (4 bytes a candidate): a warp takes a
 // strip of kStrip consecutive logits of a row and leaves its maximum and its sum
 // of exponentials, nothing else; no barrier, no shared memory, no list. A second
-// launch, one CTA per group, makes the rows' log sums (in 64 bits) and from them
-// every strip's best score. At most `beams` strips can hold a winner: those first
+// launch, one CTA per group, adds the strips' sums up in 64 bits and finds every
+// strip's best score. At most `beams` strips can hold a winner: those first
 // in the order (best score, then row and strip). Only they are read again, by a
 // warp each, and their `beams` best logits ranked by counting.
 //
-// 64 rows of 262144 (16 groups of 4): 13.5 us for the scan (10.2 at the copy
-// rate; 16384 strips are 3.5 waves of the resident warps) and 7 for the pick,
+// Precision: the exponentials (hardware ex2, 2^-22) and a strip's sum are 32-bit:
+// the scan is bound by its 4 bytes a candidate and would not be with 64-bit ones.
+// A row's logarithm is off by 1e-7 or so, the same for all its tokens; scores are
+// then put together and compared in 64 bits. Within a row that is the order of the
+// logits; continuations of different rows that lie closer than 1e-7 may change places.
+//
+// 64 rows of 262144 (16 groups of 4): 21 us, 13.3 for the scan (10.2 at the copy
+// rate; 16384 strips are 3.5 waves of the resident warps) and the rest for the pick,
 // which is latency: five steps with a barrier each. Selecting in the scan itself
 // (sorted maxima and candidates per chunk) took 32 us, a ring of chunks with a
 // running bound 33, persistent warps with the next strip in flight 26.
 //
-// Order: by the 64-bit score, ties to the lower row, then the lower token; equal
+// Order: by the score so made, ties to the lower row, then the lower token; equal
 // logits of one row have equal scores. Every comparison is on unique pairs, so
 // the result does not depend on the order in which warps arrive. A strip that is
 // not among the first `beams` holds no winner: each of those has a continuation

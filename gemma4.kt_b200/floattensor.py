@@ -110,12 +110,14 @@ class Context:
 
     def close(self) -> None:
         self.work = {}
-        for passed, _ in self.held:
-            passed.synchronize()
-        self.held.clear()
-        if self.handle:
-            lib().g4_destroy(self.handle)
-            self.handle = None
+        try:
+            for passed, _ in self.held:
+                passed.synchronize()
+        finally:
+            self.held.clear()
+            if self.handle:
+                lib().g4_destroy(self.handle)
+                self.handle = None
 
     def __del__(self):
         try:
