@@ -327,7 +327,7 @@ def test_arguments_freed_before_their_stream_ran(g4, ctx):
     assert cache.lens.tolist() == [20, 33, 40, 20, 33, 0, 0, 0]
     assert torch.equal(out, want) and torch.equal(out2, turned)
     assert all(torch.equal(a, b) for a, b in zip(best, chosen))
-    assert len(ctx.held) >= 5
+    assert ctx.held  # the last call's at least
     assert cache.check() == 64 - 3 - 2 - 3
     assert not ctx.held
 
